@@ -510,6 +510,112 @@ int mmr_reshard_plan_stats(mmr_context* ctx, mmr_store* src, mmr_store* dst, mmr
 int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_store* const* dsts, int32_t n,
                                  mmr_plan_stats* out);
 
+/* ---------------------------------------------------------------------------
+ * Page cache: keys and values of a decode mesh, in pages.  No counterpart in
+ * the reference.  What a reshard brings to a mesh is written into the pages of
+ * a cache, and the page operators move those pages about, in every pool and on
+ * every device of the mesh in one call.
+ *
+ * A cache is a set of stores the caller owns:
+ *   pools    dim 0 is the pages, unsharded and slowest in the buffers; the rest of the shape, its sharding and layout
+ *            are free (mmr_pages_write wants [pages, page_tokens, heads, dim], heads alone sharded).  Any type.
+ *   table    S32 [S, B] in one buffer: the page ids of S sequences of at most B pages
+ *   lengths  S32 [S]: tokens every sequence holds; 0: empty, its row means nothing
+ *   refs     S32 [pages]: how many sequences use a page; 0: free
+ * Zeros (a new store) are an empty cache.  The caller may read and write the tables between calls, e.g. to keep a
+ * page alive that no sequence uses (refs + 1).
+ *
+ * Arrays of sequences, pages and counts are int32 in device memory, 4-byte aligned, read when the call's kernels run:
+ * the caller orders their writes before the call on the context's stream.  Every call is asynchronous, allocates
+ * nothing, copies nothing from the host and may be captured into a HIP graph; calls of one cache are ordered by the
+ * context's stream, and graphs captured from one cache must not run at the same time, as they share its tables and
+ * workspace.  (The first call after a pool was offloaded and reloaded enters its buffers anew and is refused while
+ * capturing, and a graph captured before that must not be replayed.)
+ *
+ * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
+ * so on.  extend, fork and copy check all their entries first and change nothing at all if one is bad; the reason is
+ * kept until mmr_pages_status reads it.  Pages are given out lowest free id first, in the order of the entries.
+ * ------------------------------------------------------------------------- */
+typedef struct mmr_pages mmr_pages;
+
+#define MMR_PAGES_BAD_SEQUENCE 1u   /* a sequence outside [0, S) */
+#define MMR_PAGES_BAD_PAGE 2u       /* a page outside the pools, in an argument or in a row of the table */
+#define MMR_PAGES_OUT_OF_PAGES 4u   /* fewer free pages than the call needs */
+#define MMR_PAGES_TOO_LONG 8u       /* more tokens than a row holds, or a negative count or length */
+#define MMR_PAGES_REPEATED 16u      /* a sequence (extend, fork: child) or a destination page (copy) named twice */
+#define MMR_PAGES_NOT_EMPTY 32u     /* fork into a sequence that holds tokens */
+#define MMR_PAGES_SHARED_TAIL 64u   /* extend of a sequence whose last, partly filled page has other users */
+#define MMR_PAGES_OVERLAP 128u      /* copy: a destination is also the source of another pair */
+#define MMR_PAGES_BAD_COUNT 256u    /* free, compact: refs out of step with the table (a page in a row that nobody uses) */
+
+/* page_tokens: tokens a page holds.  At most 2^21 sequences and 2^24 pages.  The handle lives until mmr_pages_destroy or
+ * the end of the context; its stores must outlive it. */
+int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools, mmr_store* table, mmr_store* lengths,
+                     mmr_store* refs, int32_t page_tokens, mmr_pages** out);
+int mmr_pages_destroy(mmr_pages* pages);
+/* tokens[i] more tokens for sequences[i]: lengths grows, and the pages that takes are given out.  Their contents are
+ * whatever they held (mmr_pages_write fills them). */
+int mmr_pages_extend(mmr_pages* pages, const int32_t* sequences, const int32_t* tokens, int32_t n);
+/* children[i] (empty) becomes a copy of parents[i]: it shares the full pages, and gets a page of its own, copied in
+ * every pool, for a last one that is partly filled.  A parent may be named any number of times. */
+int mmr_pages_fork(mmr_pages* pages, const int32_t* parents, const int32_t* children, int32_t n);
+/* The sequences end: lengths 0, a user less for each of their pages.  Rows of the table keep their ids.  A sequence
+ * that is empty, or named a second time, is left alone; an entry outside the table is skipped, the others are freed. */
+int mmr_pages_free(mmr_pages* pages, const int32_t* sequences, int32_t n);
+/* Page destinations[i] of every pool := page sources[i].  A page may be the source of several pairs; destinations are
+ * distinct and no source of another pair.  The tables are not touched. */
+int mmr_pages_copy(mmr_pages* pages, const int32_t* sources, const int32_t* destinations, int32_t n);
+/* Moves pages so that those in use are 0 .. (pages in use - 1): the k-th page in use beyond that bound goes to the k-th
+ * free page below it.  refs moves along, and the rows of all sequences that hold tokens are renamed; ids that the caller
+ * keeps elsewhere go stale. */
+int mmr_pages_compact(mmr_pages* pages);
+/* Blocks until the cache's calls are done; *flags receives the MMR_PAGES_* reasons since the last status and clears
+ * them, *pages_in_use (may be NULL) the pages with refs > 0. */
+int mmr_pages_status(mmr_pages* pages, uint32_t* flags, int64_t* pages_in_use);
+
+/* Rotary positions.  A row's first rotary_dim elements are pairs, (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * `interleaved`; pair i at position p is turned by p * f_i radians, f_i = base^(-2 i / rotary_dim) or frequencies[i]
+ * (rotary_dim / 2 of them, read by mmr_rotary_create), and multiplied by `magnitude`.  For contexts longer than those of
+ * training: MMR_ROTARY_LINEAR divides every f_i by `factor`; MMR_ROTARY_BY_PARTS divides those that make fewer than
+ * low_turns turns over original_positions, leaves those of more than high_turns as they are, and goes over from one to
+ * the other linearly in the turns. */
+#define MMR_ROTARY_UNSCALED 0
+#define MMR_ROTARY_LINEAR 1
+#define MMR_ROTARY_BY_PARTS 2
+typedef struct {
+  int32_t rotary_dim; /* even */
+  int32_t interleaved;
+  double base;
+  int32_t scaling; /* MMR_ROTARY_* */
+  double factor;
+  int64_t original_positions;
+  double low_turns, high_turns;
+  double magnitude;          /* 1: a rotation; what long contexts multiply the attention by, else */
+  const double* frequencies; /* radians per position instead of base, or NULL */
+} mmr_rotary_options;
+typedef struct mmr_rotary mmr_rotary;
+int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* options, mmr_rotary** out);
+int mmr_rotary_destroy(mmr_rotary* rotary);
+
+/* out := x with its rows turned.  x and out: F32, BF16 or F16, rank 2 to 4, of one descriptor (out may be x itself, and
+ * overlaps it in no other way); the last dim is the row, unsharded and minor-most, at least rotary_dim long, the rest of
+ * it passes through.  Every other dim may be sharded, padded and laid out at will; padding is left alone.  The position
+ * of a row is offset + its index along seq_dim in the whole array, wherever its tile is, or what `positions` holds: an
+ * S32 store [sequence], or [dim 0, sequence], whose tile on every device covers the sequence of x's tile there (sharded
+ * alike, or replicated).  MMR_ROTARY_BACKWARD: out is the gradient of x where x holds the gradient of the result. */
+#define MMR_ROTARY_BACKWARD 1u
+int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t seq_dim, mmr_store* positions, int64_t offset,
+                     uint32_t flags);
+
+/* New tokens into the pages of a cache, after mmr_pages_extend made room for them: tokens begins[i] .. begins[i + 1] - 1
+ * of k (and v, q) are the last ones of sequences[i], so the first stands at position lengths - (begins[i + 1] -
+ * begins[i]).  begins: n + 1 ascending values; tokens before the first and after the last are padding and left out.  k
+ * goes to pool k_pool, v (or NULL) to pool v_pool: stores [tokens, heads, dim], heads sharded as in the pool.  With a
+ * rotary plan k is turned on its way, and q (any heads, [tokens, heads, dim], or NULL) is turned into q_out (or in
+ * place).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type. */
+int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* begins, int32_t n, int32_t k_pool, mmr_store* k,
+                    int32_t v_pool, mmr_store* v, mmr_rotary* rotary, mmr_store* q, mmr_store* q_out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,10 @@ MMR_PLAN_ALL_GENERIC, MMR_PLAN_NO_AUTOTUNE, MMR_PLAN_NO_SPAN = 1, 2, 4
 MMR_PLAN_NO_INLINE, MMR_PLAN_NO_SEGMENT_TABLES = 8, 16
 MMR_CHECK_INVARIANTS = 1
 MMR_STATIC_SCRATCH_BYTES = 1 << 20
+PAGES_FLAGS = {"BAD_SEQUENCE": 1, "BAD_PAGE": 2, "OUT_OF_PAGES": 4, "TOO_LONG": 8, "REPEATED": 16, "NOT_EMPTY": 32,
+               "SHARED_TAIL": 64, "OVERLAP": 128, "BAD_COUNT": 256}
+ROTARY_SCALINGS = {None: 0, "linear": 1, "parts": 2}
+MMR_ROTARY_BACKWARD = 1
 
 STATUS_NAMES = {0: "OK", 1: "INVALID_ARGUMENT", 2: "UNSUPPORTED", 3: "OUT_OF_MEMORY",
                 4: "HIP_ERROR", 5: "NOT_FOUND", 6: "INTERNAL"}
@@ -105,6 +109,12 @@ class ContextStats(C.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class RotaryOptions(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("base", C.c_double), ("scaling", C.c_int32),
+                ("factor", C.c_double), ("original_positions", C.c_int64), ("low_turns", C.c_double), ("high_turns", C.c_double),
+                ("magnitude", C.c_double), ("frequencies", C.POINTER(C.c_double))]
+
+
 # Every symbol include/mmreshard.h declares: name -> (restype, argtypes)
 P = C.POINTER
 VP = C.c_void_p
@@ -188,6 +198,18 @@ PROTOTYPES = {
     "mmr_context_get_stats": (C.c_int, [VP, P(ContextStats)]),
     "mmr_reshard_plan_stats": (C.c_int, [VP, VP, VP, P(PlanStats)]),
     "mmr_reshard_batch_plan_stats": (C.c_int, [VP, P(VP), P(VP), I32, P(PlanStats)]),
+    "mmr_pages_create": (C.c_int, [VP, P(VP), I32, VP, VP, VP, I32, P(VP)]),
+    "mmr_pages_destroy": (C.c_int, [VP]),
+    "mmr_pages_extend": (C.c_int, [VP, VP, VP, I32]),
+    "mmr_pages_fork": (C.c_int, [VP, VP, VP, I32]),
+    "mmr_pages_free": (C.c_int, [VP, VP, I32]),
+    "mmr_pages_copy": (C.c_int, [VP, VP, VP, I32]),
+    "mmr_pages_compact": (C.c_int, [VP]),
+    "mmr_pages_status": (C.c_int, [VP, P(C.c_uint32), P(I64)]),
+    "mmr_pages_write": (C.c_int, [VP, VP, VP, I32, I32, VP, I32, VP, VP, VP, VP]),
+    "mmr_rotary_create": (C.c_int, [VP, P(RotaryOptions), P(VP)]),
+    "mmr_rotary_destroy": (C.c_int, [VP]),
+    "mmr_rotary_apply": (C.c_int, [VP, VP, VP, I32, VP, I64, C.c_uint32]),
 }
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmmreshard.so")

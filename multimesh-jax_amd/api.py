@@ -328,6 +328,86 @@ class StoreHandle:
         return shard_bytes(self.shape)
 
 
+def _ids(a, what: str) -> Tuple[int, int]:
+    """(device address, entries) of an int32 array in device memory: a StoreHandle (S32, one device, rank 1), an array
+    object of a GPU framework (int32, contiguous, on the GPU), or such a pair itself."""
+    if isinstance(a, StoreHandle):
+        s = a.shape
+        if s.dtype != B.DTYPES["S32"] or s.dev_count != 1 or s.ndims != 1:
+            raise ValueError("%s: a store of ids is S32, of rank 1 and on one device" % what)
+        return a._ctx.SliceLocalShard(s.dev_start, a, wait=False), int(s.dims[0].size)
+    if hasattr(a, "data_ptr"):
+        if not getattr(a, "is_cuda", False):
+            raise ValueError("%s: the array is not in device memory" % what)
+        if not str(a.dtype).endswith(".int32") or not a.is_contiguous():
+            raise ValueError("%s: ids are int32 and contiguous, not %s" % (what, a.dtype))
+        return a.data_ptr(), a.numel()
+    if isinstance(a, tuple) and len(a) == 2:
+        return int(a[0]), int(a[1])
+    raise TypeError("%s: ids are a StoreHandle, an int32 array in device memory, or (device address, entries)" % what)
+
+
+class RotaryPlan:
+    """The angles of rotary positions (mmr_rotary_create); made by ReshardContext.CreateRotary."""
+
+    def __init__(self, ctx: "ReshardContext", handle: C.c_void_p):
+        self._ctx, self._h = ctx, handle
+
+    def Destroy(self) -> None:
+        B.check(self._ctx._lib.mmr_rotary_destroy(self._h))
+        self._h = None
+
+
+class PageCache:
+    """Pages of keys and values in a set of stores (include/mmreshard.h, "Page cache"); made by
+    ReshardContext.CreatePages.  Sequences, pages and counts are int32 arrays in device memory (see _ids).  Calls are
+    asynchronous; what an entry had wrong is told by Status."""
+
+    def __init__(self, ctx: "ReshardContext", handle: C.c_void_p):
+        self._ctx, self._h, self._lib = ctx, handle, ctx._lib
+
+    def _pairs(self, fn, a, b, what):
+        (pa, na), (pb, nb) = _ids(a, what[0]), _ids(b, what[1])
+        if na != nb:
+            raise ValueError("%d %s, %d %s" % (na, what[0], nb, what[1]))
+        B.check(fn(self._h, pa, pb, na))
+
+    def Extend(self, sequences, tokens) -> None:
+        self._pairs(self._lib.mmr_pages_extend, sequences, tokens, ("sequences", "tokens"))
+
+    def Fork(self, parents, children) -> None:
+        self._pairs(self._lib.mmr_pages_fork, parents, children, ("parents", "children"))
+
+    def Free(self, sequences) -> None:
+        p, n = _ids(sequences, "sequences")
+        B.check(self._lib.mmr_pages_free(self._h, p, n))
+
+    def Copy(self, sources, destinations) -> None:
+        self._pairs(self._lib.mmr_pages_copy, sources, destinations, ("sources", "destinations"))
+
+    def Compact(self) -> None:
+        B.check(self._lib.mmr_pages_compact(self._h))
+
+    def Write(self, sequences, begins, k_pool: int, k: StoreHandle, v_pool: int = -1, v: Optional[StoreHandle] = None,
+              rotary: Optional[RotaryPlan] = None, q: Optional[StoreHandle] = None, q_out: Optional[StoreHandle] = None) -> None:
+        """New tokens into the pages (mmr_pages_write); `begins` has an entry more than `sequences`."""
+        (ps, n), (pb, nb) = _ids(sequences, "sequences"), _ids(begins, "begins")
+        if nb != n + 1:
+            raise ValueError("%d begins for %d sequences" % (nb, n))
+        h = lambda s: s._h if s is not None else None  # noqa: E731
+        B.check(self._lib.mmr_pages_write(self._h, ps, pb, n, k_pool, k._h, v_pool, h(v), h(rotary), h(q), h(q_out)))
+
+    def Status(self) -> Tuple[List[str], int]:
+        """(reasons since the last Status, pages in use).  Blocks."""
+        flags, used = C.c_uint32(), C.c_int64()
+        B.check(self._lib.mmr_pages_status(self._h, C.byref(flags), C.byref(used)))
+        return [name for name, bit in B.PAGES_FLAGS.items() if flags.value & bit], used.value
+
+    def Destroy(self) -> None:
+        B.check(self._lib.mmr_pages_destroy(self._h))
+        self._h = None
+
+
 class ReshardContext:
     """Store subset of xla::ZukuExecuteContext on one MI355X.
 
@@ -501,6 +581,35 @@ class ReshardContext:
 
     def Sync(self) -> None:
         B.check(self._lib.mmr_sync(self._h))
+
+    # -- pages and rotary positions -----------------------------------------
+    def CreatePages(self, pools: Sequence[StoreHandle], table: StoreHandle, lengths: StoreHandle, refs: StoreHandle,
+                    page_tokens: int) -> PageCache:
+        h = C.c_void_p()
+        arr = (C.c_void_p * max(len(pools), 1))(*[p._h for p in pools])
+        B.check(self._lib.mmr_pages_create(self._h, arr, len(pools), table._h, lengths._h, refs._h, page_tokens, C.byref(h)))
+        return PageCache(self, h)
+
+    def CreateRotary(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: Optional[str] = None,
+                     factor: float = 1.0, original_positions: int = 0, low_turns: float = 0.0, high_turns: float = 0.0,
+                     magnitude: float = 1.0, frequencies: Optional[Sequence[float]] = None) -> RotaryPlan:
+        """scaling: None, "linear" or "parts" (mmr_rotary_options); frequencies: radians per position of every pair."""
+        o = B.RotaryOptions(rotary_dim, int(interleaved), base, B.ROTARY_SCALINGS[scaling], factor, original_positions, low_turns,
+                            high_turns, magnitude, None)
+        if frequencies is not None:
+            if len(frequencies) * 2 != rotary_dim:
+                raise ValueError("%d frequencies for %d elements" % (len(frequencies), rotary_dim))
+            o.frequencies = (C.c_double * max(len(frequencies), 1))(*frequencies)
+        h = C.c_void_p()
+        B.check(self._lib.mmr_rotary_create(self._h, C.byref(o), C.byref(h)))
+        return RotaryPlan(self, h)
+
+    def ApplyRotary(self, rotary: RotaryPlan, x: StoreHandle, out: Optional[StoreHandle] = None, seq_dim: int = 0,
+                    positions: Optional[StoreHandle] = None, offset: int = 0, backward: bool = False) -> None:
+        """Rows of x turned by their positions, into `out` (None: in place)."""
+        B.check(self._lib.mmr_rotary_apply(rotary._h, x._h, (out if out is not None else x)._h, seq_dim,
+                                           positions._h if positions is not None else None, offset,
+                                           B.MMR_ROTARY_BACKWARD if backward else 0))
 
     # -- measurement and inspection ----------------------------------------
     def set_plan_options(self, chunk_bytes: int = 0, order: int = 0, xcd_mode: int = 0, flags: int = 0) -> None:

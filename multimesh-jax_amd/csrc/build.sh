@@ -10,12 +10,14 @@ hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared \
   -Wall -Wextra -Wno-unused-command-line-argument -DMMR_SOURCE_DIGEST="\"${digest}\"" ${MMR_EXTRA_FLAGS:-} \
   -I"${here}/../../include" -I"${here}" \
   "${here}/geometry.cc" "${here}/sharding_frontend.cc" "${here}/planner.cc" \
-  "${here}/context.cc" "${here}/hip_execute_context.cc" "${here}/shard_buffer.cc" "${here}/kernels.hip" \
+  "${here}/context.cc" "${here}/hip_execute_context.cc" "${here}/shard_buffer.cc" "${here}/page_cache.cc" \
+  "${here}/kernels.hip" "${here}/page_kernels.hip" \
   -o "${out}"
 # no kernel may touch scratch memory (a lane-indexed local array would put it there and cost most of the bandwidth)
-usage="$(hipcc --offload-arch=gfx950 -O3 -std=c++17 --cuda-device-only -c -o /dev/null \
+usage="$(for f in kernels.hip page_kernels.hip; do
+  hipcc --offload-arch=gfx950 -O3 -std=c++17 --cuda-device-only -c -o /dev/null \
   -Xclang -target-feature -Xclang -packed-fp32-ops -Rpass-analysis=kernel-resource-usage ${MMR_EXTRA_FLAGS:-} \
-  -I"${here}/../../include" -I"${here}" "${here}/kernels.hip" 2>&1 | grep -E "Function Name|ScratchSize|VGPRs:|Occupancy" || true)"
+  -I"${here}/../../include" -I"${here}" "${here}/${f}" 2>&1 | grep -E "Function Name|ScratchSize|VGPRs:|Occupancy" || true; done)"
 echo "${usage}" | sed 's/^.*remark: /  /'
 if echo "${usage}" | grep -E "ScratchSize \[bytes/lane\]: [1-9]" >/dev/null; then
   echo "error: a kernel uses scratch memory" >&2

@@ -27,6 +27,7 @@
 
 #include "common.h"
 #include "chunk_ops.h"
+#include "context_access.h"
 #include "kernels.h"
 #include "planner.h"
 
@@ -264,6 +265,8 @@ struct mmr_context {
   std::unordered_map<size_t, std::vector<char*>> free_pool;
   size_t free_pool_bytes = 0;
   std::unordered_map<int64_t, std::unique_ptr<mmr_store>> stores;
+  uint64_t store_epoch = 0;  // bumped when a store is freed, offloaded or reloaded
+  std::unordered_map<mmr::Attachment*, std::unique_ptr<mmr::Attachment>> attachments;  // handles of other operators
   int64_t next_ordinal = 0;
   mmr_context_stats stats{};
   // mmr_reshard_batch_static: this GPU's static scratch array, a pinned staging buffer of the same size and the event
@@ -1253,6 +1256,43 @@ int tile_index(const mmr_store* s, int64_t device, int64_t* k) {
 
 }  // namespace
 
+namespace mmr {
+
+ContextLock::ContextLock(mmr_context* ctx) : lock_(ctx->mu) { note_work(ctx); }
+int context_use_device(mmr_context* ctx) { return use_device(ctx); }
+hipStream_t context_stream(mmr_context* ctx) { return ctx->stream; }
+int context_refuse_capture(mmr_context* ctx, const char* what) { return refuse_capture(ctx, what); }
+int context_wait(mmr_context* ctx) { return blocking_sync(ctx); }
+void context_count(mmr_context* ctx, int64_t launches) { ctx->stats.kernel_launches += launches; }
+void context_hash(mmr_context* ctx, uint64_t kind, std::initializer_list<uint64_t> values) { hash_op(ctx, kind, values); }
+int context_take_block(mmr_context* ctx, size_t bytes, char** out, size_t* capacity) { return take_block(ctx, bytes, out, capacity); }
+void context_give_block(mmr_context* ctx, char* block, size_t capacity) { give_block(ctx, block, capacity); }
+int context_upload(mmr_context* ctx, void* device, const void* host, size_t bytes) { return staged_upload(ctx, device, host, bytes); }
+void context_attach(mmr_context* ctx, std::unique_ptr<Attachment> a) {
+  Attachment* key = a.get();
+  key->owner = ctx;
+  ctx->attachments.emplace(key, std::move(a));
+}
+void context_detach(mmr_context* ctx, Attachment* a) { ctx->attachments.erase(a); }
+uint64_t context_store_epoch(mmr_context* ctx) { return ctx->store_epoch; }
+mmr_store* context_find_store(mmr_context* ctx, int64_t id) {
+  auto it = ctx->stores.find(id);
+  return it == ctx->stores.end() ? nullptr : it->second.get();
+}
+int context_check_store(mmr_context* ctx, const mmr_store* store, const char* what) {
+  if (int rc = check_store(ctx, store, what)) return rc;
+  if (store->offloaded())
+    return fail(MMR_INVALID_ARGUMENT, "%s store %lld is offloaded to host memory", what, (long long)store->id);
+  return MMR_OK;
+}
+const Side& store_side(const mmr_store* store) { return store->side; }
+const mmr_sharded_shape& store_shape(const mmr_store* store) { return store->shape; }
+const std::string& store_key(const mmr_store* store) { return store->shape_key; }
+int64_t store_ordinal(const mmr_store* store) { return store->ordinal; }
+char* store_tile(const mmr_store* store, int64_t k) { return store->tile(k); }
+
+}  // namespace mmr
+
 extern "C" {
 
 int mmr_context_create(int32_t hip_device, void* hip_stream, mmr_context** out) {
@@ -1310,6 +1350,7 @@ void mmr_context_destroy(mmr_context* ctx) {
     ctx->callback_thread.join();
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);  // work the last callbacks queued
   }
+  ctx->attachments.clear();  // their blocks go to the block pool too
   for (auto& b : ctx->bindings) give_block(ctx, b->d_block, b->capacity);
   ctx->bindings.clear();
   ctx->binding_index.clear();
@@ -1502,6 +1543,7 @@ int mmr_store_free(mmr_context* ctx, mmr_store* store, int32_t keep_in_cache) {
     ctx->stats.bytes_allocated -= static_cast<int64_t>(store->bytes);
   }
   ctx->stats.stores_live -= 1;
+  ctx->store_epoch += 1;
   ctx->stores.erase(store->id);
   return MMR_OK;
 }
@@ -1708,6 +1750,7 @@ int mmr_store_offload(mmr_context* ctx, mmr_store* store) {
     return fail(MMR_HIP_ERROR, "copy of store %lld to host memory failed: %s", (long long)store->id, hipGetErrorString(e));
   }
   store->host = host;
+  ctx->store_epoch += 1;
   ctx->buffer_cache[store->shape_key].push_back(CachedBuffer{store->base, store->bytes});
   store->base = nullptr;
   return MMR_OK;
@@ -1738,6 +1781,7 @@ int mmr_store_reload(mmr_context* ctx, mmr_store* store) {
     return fail(MMR_HIP_ERROR, "copy of store %lld back to the device failed: %s", (long long)store->id, hipGetErrorString(e));
   }
   store->base = base;
+  ctx->store_epoch += 1;
   // the pinned buffer goes to the host cache at once: the next offload into it is ordered behind this copy
   ctx->host_cache[store->shape_key].push_back(CachedBuffer{store->host, store->bytes});
   store->host = nullptr;

@@ -1,0 +1,252 @@
+// gfx950 kernels of the page cache and of rotary positions.  What a workgroup does stands in page_ops.h and
+// rotary_ops.h, shared with the host emulation of the tests; here is how a workgroup synchronises, and the launches.
+#include <hip/hip_runtime.h>
+
+#include "device_mem.h"
+#include "page_kernels.h"
+
+namespace mmr {
+namespace {
+
+typedef DeviceMem<true, true> StreamMem;  // page moves: every byte is touched once
+typedef DeviceMem<false, false> CachedMem;
+
+// A workgroup of K threads.
+template <int K>
+struct Workgroup {
+  static constexpr int kThreads = K;
+  int32_t tid;
+  uint32_t block, blocks;
+  int32_t* shared;  // K / 64 + 1 words for the scan
+
+  __device__ __forceinline__ Workgroup(int32_t* lds) : tid(threadIdx.x), block(blockIdx.x), blocks(gridDim.x), shared(lds) {}
+  __device__ __forceinline__ void sync() { __syncthreads(); }
+
+  __device__ __forceinline__ void load4(const int32_t* p, int32_t at, int32_t n, int32_t (&r)[4]) {
+    if (at + 3 < n) {
+      const int4 v = *reinterpret_cast<const int4*>(p + at);  // the buffer and `at` are 16-byte aligned
+      r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = at + i < n ? p[at + i] : 1;
+    }
+  }
+
+  template <class V>
+  __device__ __forceinline__ V scan(V v, V* total) {
+    V* sums = reinterpret_cast<V*>(shared);
+    const int lane = tid & 63, wave = tid >> 6;
+    V in = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const V other = __shfl_up(in, d, 64);
+      if (lane >= d) in += other;
+    }
+    if (lane == 63) sums[wave] = in;
+    __syncthreads();
+    V before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < K / 64; ++i) {
+      const V s = sums[i];
+      before += i < wave ? s : 0;
+      all += s;
+    }
+    __syncthreads();
+    *total = all;
+    return before + in - v;
+  }
+
+  __device__ __forceinline__ uint32_t any(uint32_t flags) {
+    if (tid == 0) shared[0] = 0;
+    __syncthreads();
+    if (flags) atomicOr(&shared[0], static_cast<int32_t>(flags));
+    __syncthreads();
+    const uint32_t all = static_cast<uint32_t>(shared[0]);
+    __syncthreads();
+    return all;
+  }
+
+  __device__ __forceinline__ int32_t atomic_add(int32_t* p, int32_t v) { return atomicAdd(p, v); }
+  __device__ __forceinline__ int32_t atomic_exch(int32_t* p, int32_t v) { return atomicExch(p, v); }
+  __device__ __forceinline__ void atomic_or(int32_t* p, int32_t v) { atomicOr(p, v); }
+
+  // True in the workgroup that arrives last, which then sees what all others wrote (their L2 may be another XCD's: the
+  // fences write it back and drop what is stale).  The counter is zero again for the next launch.
+  __device__ __forceinline__ bool last_block(int32_t* counter) {
+    if (blocks == 1) {
+      __syncthreads();
+      return true;
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      const int32_t arrived = atomicAdd(counter, 1);
+      const bool last = arrived == static_cast<int32_t>(blocks) - 1;
+      if (last) atomicExch(counter, 0);
+      shared[0] = last;
+    }
+    __syncthreads();
+    const bool last = shared[0] != 0;
+    __syncthreads();
+    if (last) __threadfence();
+    return last;
+  }
+};
+
+constexpr int kScanInts = 2 * (kPagePlanThreads / 64) + 2;
+typedef Workgroup<kPagePlanThreads> PlanGroup;
+typedef Workgroup<kPageThreads> ApplyGroup;
+
+#define MMR_PLAN_SHARED                                              \
+  __shared__ __attribute__((aligned(16))) int32_t scan[kScanInts];   \
+  __shared__ int32_t prefix[kMaxPageSegments];                       \
+  PlanGroup x(scan)
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_extend_kernel(PageState st, PageWork w, const int32_t* slots,
+                                                                           const int32_t* counts, int32_t n) {
+  MMR_PLAN_SHARED;
+  page_extend(x, st, w, prefix, slots, counts, n);
+}
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_fork_plan_kernel(PageState st, PageWork w, const int32_t* parents,
+                                                                              const int32_t* children, int32_t n) {
+  MMR_PLAN_SHARED;
+  page_fork_plan(x, st, w, prefix, parents, children, n);
+}
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_compact_plan_kernel(PageState st, PageWork w) {
+  MMR_PLAN_SHARED;
+  page_compact_plan(x, st, w, prefix);
+}
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_count_kernel(PageState st, PageWork w) {
+  MMR_PLAN_SHARED;
+  page_count(x, st, w, prefix);
+}
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_copy_plan_kernel(PageState st, PageWork w, const int32_t* src,
+                                                                              const int32_t* dst, int32_t n) {
+  __shared__ __attribute__((aligned(16))) int32_t scan[kScanInts];
+  PlanGroup x(scan);
+  page_copy_plan(x, st, w, src, dst, n);
+}
+
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_free_kernel(PageState st, PageWork w, const int32_t* slots) {
+  __shared__ __attribute__((aligned(16))) int32_t scan[kScanInts];
+  PlanGroup x(scan);
+  page_free(x, st, w, scan, slots);
+}
+
+// The first `row_blocks` workgroups write tables (KIND 1: fork, 2: compact; 0: none), the others move pages.
+template <int KIND, bool ALIGNED>
+__global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState st, PageWork w, PageMover mv,
+                                                                      const int32_t* parents, const int32_t* children, int32_t n,
+                                                                      uint32_t row_blocks) {
+  if (!w.header[kPageOk]) return;
+  if (KIND != 0 && blockIdx.x < row_blocks) {
+    __shared__ __attribute__((aligned(16))) int32_t scan[2 * (kPageThreads / 64) + 2];
+    ApplyGroup x(scan);
+    if (KIND == 1) page_fork_rows(x, st, w, parents, children, n, blockIdx.x, row_blocks);
+    else page_compact_rows(x, st, w, blockIdx.x, row_blocks);
+    return;
+  }
+  const uint32_t items = static_cast<uint32_t>(w.header[kPageMoves]) * mv.n_buffers * mv.chunks;
+  const uint32_t step = gridDim.x - row_blocks;
+  for (uint32_t item = blockIdx.x - row_blocks; item < items; item += step)
+    page_move_chunk<StreamMem, ALIGNED>(mv, w.moves, item, threadIdx.x);
+}
+
+template <class T, int VEC, bool INTERLEAVED>
+__global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(RotaryArgs a) {
+  __shared__ __attribute__((aligned(16))) int32_t scan[2 * (kRotaryThreads / 64) + 2];
+  Workgroup<kRotaryThreads> x(scan);
+  const RotaryJob& j = a.jobs[blockIdx.y];
+  if (x.block >= j.blocks) return;  // uniform over the workgroup
+  rotary_block<CachedMem, T, VEC, INTERLEAVED>(x, a, j);
+}
+
+uint32_t segments(const PageWork& w) { return static_cast<uint32_t>(w.n_segments); }
+
+// Workgroups of a move: one per chunk up to this many, which then loop.
+constexpr uint64_t kMaxMoveBlocks = 1u << 18;
+
+template <int KIND>
+hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
+                        const int32_t* children, int32_t n, uint32_t row_blocks, hipStream_t stream) {
+  const uint64_t items = static_cast<uint64_t>(mv.max_moves) * mv.mover.n_buffers * mv.mover.chunks;
+  const uint32_t movers = static_cast<uint32_t>(items < kMaxMoveBlocks ? items : kMaxMoveBlocks);
+  if (movers + row_blocks == 0) return hipSuccess;
+  if (mv.aligned)
+    hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, true>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
+                       mv.mover, parents, children, n, row_blocks);
+  else
+    hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, false>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
+                       mv.mover, parents, children, n, row_blocks);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_page_extend(const PageState& st, const PageWork& w, const int32_t* slots, const int32_t* counts, int32_t n,
+                              hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_extend_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w, slots, counts, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_t* slots, int32_t n, hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_free_kernel, dim3(static_cast<uint32_t>(n)), dim3(kPagePlanThreads), 0, stream, st, w, slots);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_fork(const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children, int32_t n,
+                            const PageMoveLaunch& mv, hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_fork_plan_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w, parents, children, n);
+  if (hipError_t e = hipGetLastError()) return e;
+  return launch_apply<1>(st, w, mv, parents, children, n, static_cast<uint32_t>(n < 4096 ? n : 4096), stream);
+}
+
+hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_compact_plan_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w);
+  if (hipError_t e = hipGetLastError()) return e;
+  return launch_apply<2>(st, w, mv, nullptr, nullptr, 0, static_cast<uint32_t>(st.S < 4096 ? st.S : 4096), stream);
+}
+
+hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
+                            const PageMoveLaunch& mv, hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_copy_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, src, dst, n);
+  if (hipError_t e = hipGetLastError()) return e;
+  return launch_apply<0>(st, w, mv, nullptr, nullptr, 0, 0, stream);
+}
+
+hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream) {
+  hipLaunchKernelGGL(mmr_page_count_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w);
+  return hipGetLastError();
+}
+
+hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, hipStream_t stream) {
+  uint32_t blocks = 0;
+  for (int i = 0; i < n_jobs; ++i) blocks = args.jobs[i].blocks > blocks ? args.jobs[i].blocks : blocks;
+  if (!blocks) return hipSuccess;
+  const dim3 grid(blocks, static_cast<uint32_t>(n_jobs)), threads(kRotaryThreads);
+#define MMR_ROTARY(T, V, I) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I>), grid, threads, 0, stream, args)
+#define MMR_ROTARY_TYPE(T, V)                                     \
+  do {                                                            \
+    if (vectors && interleaved) MMR_ROTARY(T, V, true);           \
+    else if (vectors) MMR_ROTARY(T, V, false);                    \
+    else if (interleaved) MMR_ROTARY(T, 1, true);                 \
+    else MMR_ROTARY(T, 1, false);                                 \
+  } while (0)
+  switch (type) {
+    case MMR_F32: MMR_ROTARY_TYPE(RotaryF32, 4); break;
+    case MMR_BF16: MMR_ROTARY_TYPE(RotaryBF16, 8); break;
+    case MMR_F16: MMR_ROTARY_TYPE(RotaryF16, 8); break;
+    default:
+      if (vectors) MMR_ROTARY(RotaryRaw, 16, false);
+      else MMR_ROTARY(RotaryRaw, 1, false);
+  }
+#undef MMR_ROTARY_TYPE
+#undef MMR_ROTARY
+  return hipGetLastError();
+}
+
+}  // namespace mmr

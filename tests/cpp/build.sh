@@ -35,3 +35,12 @@ g++ -O1 -g -std=c++17 -fsanitize=address,undefined -fno-sanitize-recover=undefin
   "${root}/multimesh-jax_amd/csrc/planner.cc" "${here}/kernel_emulation.cc" "${here}/sanitize_sweep.cc" \
   -o "${here}/sanitize_sweep"
 echo "built ${here}/sanitize_sweep"
+# The page-cache and rotary kernels with host threads as the lanes of a workgroup, under the sanitizers (clang: g++ 11 has no
+# 16-bit float types).
+clang="${ROCM_PATH:-/opt/rocm}/llvm/bin/clang++"
+"${clang}" -O1 -g -std=c++20 -fsanitize=address,undefined -fno-sanitize-recover=undefined -fno-omit-frame-pointer -Wall -Wextra \
+  -Wno-unknown-pragmas -I"${root}/include" -I"${root}/multimesh-jax_amd/csrc" "${here}/page_sweep.cc" -pthread -o "${here}/page_sweep"
+echo "built ${here}/page_sweep"
+"${clang}" -O1 -g -std=c++20 -fsanitize=thread -Wall -Wextra -Wno-unknown-pragmas -I"${root}/include" \
+  -I"${root}/multimesh-jax_amd/csrc" "${here}/page_sweep.cc" -pthread -o "${here}/page_sweep_threads"
+echo "built ${here}/page_sweep_threads"
