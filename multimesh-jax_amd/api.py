@@ -328,20 +328,30 @@ class StoreHandle:
         return shard_bytes(self.shape)
 
 
+_INT32_TYPES: dict = {}  # type objects of other packages -> whether they are int32 (their names are slow to make)
+
+
+def _is_int32(dtype) -> bool:
+    known = _INT32_TYPES.get(dtype)
+    if known is None:
+        known = _INT32_TYPES[dtype] = str(dtype).rsplit(".", 1)[-1] == "int32"
+    return known
+
+
 def _ids(a, what: str) -> Tuple[int, int]:
     """(device address, entries) of an int32 array in device memory: a StoreHandle (S32, one device, rank 1), an array
     object of a GPU framework (int32, contiguous, on the GPU), or such a pair itself."""
+    if hasattr(a, "data_ptr"):
+        if not getattr(a, "is_cuda", False):
+            raise ValueError("%s: the array is not in device memory" % what)
+        if not _is_int32(a.dtype) or not a.is_contiguous():
+            raise ValueError("%s: ids are int32 and contiguous, not %s" % (what, a.dtype))
+        return a.data_ptr(), a.numel()
     if isinstance(a, StoreHandle):
         s = a.shape
         if s.dtype != B.DTYPES["S32"] or s.dev_count != 1 or s.ndims != 1:
             raise ValueError("%s: a store of ids is S32, of rank 1 and on one device" % what)
         return a._ctx.SliceLocalShard(s.dev_start, a, wait=False), int(s.dims[0].size)
-    if hasattr(a, "data_ptr"):
-        if not getattr(a, "is_cuda", False):
-            raise ValueError("%s: the array is not in device memory" % what)
-        if not str(a.dtype).endswith(".int32") or not a.is_contiguous():
-            raise ValueError("%s: ids are int32 and contiguous, not %s" % (what, a.dtype))
-        return a.data_ptr(), a.numel()
     if isinstance(a, tuple) and len(a) == 2:
         return int(a[0]), int(a[1])
     raise TypeError("%s: ids are a StoreHandle, an int32 array in device memory, or (device address, entries)" % what)

@@ -162,9 +162,9 @@ int check_rotary(mmr_context* ctx, const mmr_rotary* r, int64_t dim, int32_t dty
   return MMR_OK;
 }
 
-// Whole 16-byte vectors throughout: the two halves of the rotated part, the row and every stride.
-bool vector_rows(int64_t rotated, int64_t dim, int itemsize) {
-  return (rotated / 2 * itemsize) % 16 == 0 && (dim * itemsize) % 16 == 0;
+// Whole 16-byte vectors throughout: the rotated part (its two halves, unless interleaved), the row and every stride.
+bool vector_rows(int64_t rotated, bool interleaved, int64_t dim, int itemsize) {
+  return ((interleaved ? rotated : rotated / 2) * itemsize) % 16 == 0 && (dim * itemsize) % 16 == 0;
 }
 
 constexpr uint64_t kMaxRotaryBlocks = (1u << 24) - 1;  // a grid has fewer than 2^32 threads
@@ -174,7 +174,10 @@ struct RotaryLaunch {
   std::vector<mmr::RotaryJob> jobs;
   int type = -1;
   bool vectors = false, interleaved = false;
+  int64_t bytes = 0;  // written
 };
+
+constexpr int64_t kL2Bytes = int64_t{32} << 20;  // eight XCDs of 4 MiB
 
 void set_plan(RotaryLaunch* l, const mmr_rotary* r, bool backward) {
   if (!r) return;
@@ -194,8 +197,11 @@ int shape_jobs(RotaryLaunch* l, const std::vector<int64_t>& dims, const std::vec
   for (size_t i = 0; i < l->jobs.size(); ++i) {
     const int64_t rot = turned[i] ? static_cast<int64_t>(l->args.half) : 0;
     const int64_t rest = turned[i] == 2 ? 0 : dims[i] * per - 2 * rot;  // 2: in place, what is not turned stays
-    units.push_back({static_cast<uint32_t>(rot / vec), static_cast<uint32_t>(rest / vec)});
-    lanes += static_cast<int64_t>(l->jobs[i].tokens) * l->jobs[i].heads * (units[i].first + units[i].second);
+    const bool one = l->interleaved && l->vectors;  // a unit is one vector, not two
+    units.push_back({static_cast<uint32_t>((one ? 2 * rot : rot) / vec), static_cast<uint32_t>(rest / vec)});
+    const int64_t rows = static_cast<int64_t>(l->jobs[i].tokens) * l->jobs[i].heads;
+    lanes += rows * (units[i].first + units[i].second);
+    l->bytes += rows * dims[i] * itemsize;
   }
   const bool spread = lanes < 256 * 1024;  // a lane each would leave the 256 CUs under four workgroups
   for (size_t i = 0; i < l->jobs.size(); ++i) {
@@ -210,7 +216,8 @@ int launch_jobs(mmr_context* ctx, RotaryLaunch* l) {
   for (size_t at = 0; at < l->jobs.size(); at += mmr::kRotaryMaxJobs) {
     const int n = static_cast<int>(std::min<size_t>(mmr::kRotaryMaxJobs, l->jobs.size() - at));
     std::copy(l->jobs.begin() + at, l->jobs.begin() + at + n, l->args.jobs);
-    MMR_HIP(mmr::launch_rotary(l->args, n, l->type, l->vectors, l->interleaved, mmr::context_stream(ctx)));
+    MMR_HIP(mmr::launch_rotary(l->args, n, l->type, l->vectors, l->interleaved, l->bytes > kL2Bytes,
+                               mmr::context_stream(ctx)));
     mmr::context_count(ctx, 1);
   }
   return MMR_OK;
@@ -274,7 +281,7 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
     return here;
   };
   const size_t header = take(mmr::kPageHeaderInts, 4), mark = take(std::max(S, P), 4), cleared = at;
-  const size_t seg_free = take(segments, 4), free_ids = take(ids, 4), live_ids = take(ids, 4), len = take(S, 4), rank = take(S, 4);
+  const size_t seg_free = take(segments, 4), seg_before = take(segments, 4), free_ids = take(ids, 4), live_ids = take(ids, 4), len = take(S, 4), rank = take(S, 4);
   const size_t moves = take(std::max(S, P), sizeof(mmr::PageMove)), map = take(P, 4);
   p->buffers_at = take(buffers, sizeof(mmr::PageBuffer));
   p->owner = ctx;
@@ -282,15 +289,14 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
   MMR_HIP(hipMemsetAsync(p->block, 0, cleared, mmr::context_stream(ctx)));
   if (int rc = upload_buffers(ctx, p.get())) return rc;
   auto ints = [&](size_t offset) { return reinterpret_cast<int32_t*>(p->block + offset); };
-  p->work = {ints(header), ints(seg_free), ints(free_ids), ints(live_ids), ints(mark), ints(len), ints(rank),
+  p->work = {ints(header), ints(seg_free), ints(seg_before), ints(free_ids), ints(live_ids), ints(mark), ints(len), ints(rank),
              reinterpret_cast<mmr::PageMove*>(p->block + moves), ints(map), static_cast<int32_t>(segments)};
   const int64_t capacity = std::min<int64_t>(B * page_tokens, 0x7fffffff);
   p->state = {reinterpret_cast<int32_t*>(mmr::store_tile(table, 0)), reinterpret_cast<int32_t*>(mmr::store_tile(lengths, 0)),
               reinterpret_cast<int32_t*>(mmr::store_tile(refs, 0)), static_cast<int32_t>(S), static_cast<int32_t>(B),
               static_cast<int32_t>(P), page_tokens, static_cast<int32_t>(capacity), mmr::make_fastdiv(static_cast<uint32_t>(page_tokens))};
   p->move.mover = {reinterpret_cast<const mmr::PageBuffer*>(p->block + p->buffers_at), static_cast<uint32_t>(buffers),
-                   static_cast<uint32_t>(chunks), mmr::make_fastdiv(static_cast<uint32_t>(chunks)),
-                   mmr::make_fastdiv(static_cast<uint32_t>(buffers))};
+                   static_cast<uint32_t>(chunks), mmr::make_fastdiv(static_cast<uint32_t>(chunks))};
   p->move.aligned = aligned;
   p->table_id = mmr_store_id(table), p->lengths_id = mmr_store_id(lengths), p->refs_id = mmr_store_id(refs);
   p->epoch = mmr::context_store_epoch(ctx);
@@ -489,7 +495,7 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
   RotaryLaunch l;
   set_plan(&l, rotary, flags & MMR_ROTARY_BACKWARD);
   l.type = s.dtype;
-  l.vectors = vector_rows(rotary->dim, s.size[s.rank - 1], s.itemsize);
+  l.vectors = vector_rows(rotary->dim, rotary->interleaved, s.size[s.rank - 1], s.itemsize);
   std::vector<int64_t> dims;
   std::vector<int> turned;
   for (int64_t k = 0; k < s.dev_count; ++k) {
@@ -589,7 +595,7 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
       dims.push_back(d.size[2]);
       turned.push_back(!turn ? 0 : j.src == j.dst ? 2 : 1);
     }
-    vectors &= vector_rows(turn ? rotary->dim : 0, d.size[2], d.itemsize);
+    vectors &= vector_rows(turn ? rotary->dim : 0, l.interleaved, d.size[2], d.itemsize);
   };
   auto add_pool = [&](const mmr_store* s, int32_t pool, bool turn, const char* what) {
     if (int rc = check_new(s, what)) return rc;

@@ -30,8 +30,9 @@ hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_
                             const PageMoveLaunch& mv, hipStream_t stream);
 hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream);
 
-// `type`: MMR_F32, MMR_BF16 or MMR_F16; -1: rows only move (no job turns anything).
-hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, hipStream_t stream);
+// `type`: MMR_F32, MMR_BF16 or MMR_F16; -1: rows only move (no job turns anything).  past_caches: how results are stored.
+hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, bool past_caches,
+                         hipStream_t stream);
 
 }  // namespace mmr
 

@@ -8,8 +8,7 @@
 namespace mmr {
 namespace {
 
-typedef DeviceMem<true, true> StreamMem;  // page moves: every byte is touched once
-typedef DeviceMem<false, false> CachedMem;
+typedef DeviceMem<true, true> StreamMem;  // every byte is touched once
 
 // A workgroup of K threads.
 template <int K>
@@ -66,31 +65,23 @@ struct Workgroup {
     return all;
   }
 
+  __device__ __forceinline__ bool all(bool v) { return __all(v); }  // over the wave
+
+  // Of n ascending values, how many are at most t; t and the call are uniform over the wave.
+  __device__ __forceinline__ int32_t ended(const int32_t* ends, int32_t n, int32_t t) {
+    int32_t count = 0;
+    for (int32_t base = 0; base < n; base += 64) {
+      const int32_t i = base + (tid & 63);
+      const uint64_t below = __ballot(i < n && ends[i < n ? i : n - 1] <= t);
+      count += __popcll(below);
+      if (~below) break;
+    }
+    return count;
+  }
+
   __device__ __forceinline__ int32_t atomic_add(int32_t* p, int32_t v) { return atomicAdd(p, v); }
   __device__ __forceinline__ int32_t atomic_exch(int32_t* p, int32_t v) { return atomicExch(p, v); }
   __device__ __forceinline__ void atomic_or(int32_t* p, int32_t v) { atomicOr(p, v); }
-
-  // True in the workgroup that arrives last, which then sees what all others wrote (their L2 may be another XCD's: the
-  // fences write it back and drop what is stale).  The counter is zero again for the next launch.
-  __device__ __forceinline__ bool last_block(int32_t* counter) {
-    if (blocks == 1) {
-      __syncthreads();
-      return true;
-    }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      const int32_t arrived = atomicAdd(counter, 1);
-      const bool last = arrived == static_cast<int32_t>(blocks) - 1;
-      if (last) atomicExch(counter, 0);
-      shared[0] = last;
-    }
-    __syncthreads();
-    const bool last = shared[0] != 0;
-    __syncthreads();
-    if (last) __threadfence();
-    return last;
-  }
 };
 
 constexpr int kScanInts = 2 * (kPagePlanThreads / 64) + 2;
@@ -102,10 +93,32 @@ typedef Workgroup<kPageThreads> ApplyGroup;
   __shared__ int32_t prefix[kMaxPageSegments];                       \
   PlanGroup x(scan)
 
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_scan_kernel(PageState st, PageWork w, bool live) {
+  __shared__ __attribute__((aligned(16))) int32_t scan[kScanInts];
+  PlanGroup x(scan);
+  page_scan_segment(x, st, w, static_cast<int32_t>(x.block), live);
+}
+
 __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_extend_kernel(PageState st, PageWork w, const int32_t* slots,
-                                                                           const int32_t* counts, int32_t n) {
+                                                                           const int32_t* counts, int32_t n, bool whole) {
   MMR_PLAN_SHARED;
-  page_extend(x, st, w, prefix, slots, counts, n);
+  page_extend_plan(x, st, w, prefix, slots, counts, n, whole);
+}
+
+#define MMR_ROWS_SHARED                                                                    \
+  __shared__ __attribute__((aligned(16))) int32_t scan[2 * (kPageThreads / 64) + 2];       \
+  __shared__ int32_t prefix[kMaxPageSegments];                                             \
+  ApplyGroup x(scan)
+
+__global__ __launch_bounds__(kPageThreads) void mmr_page_extend_rows_kernel(PageState st, PageWork w, const int32_t* slots,
+                                                                            const int32_t* counts, int32_t n) {
+  MMR_ROWS_SHARED;
+  page_extend_rows<ApplyGroup, kPageSegment>(x, st, w, prefix, slots, counts, n);
+}
+
+__global__ __launch_bounds__(kPageThreads) void mmr_page_compact_list_kernel(PageState st, PageWork w) {
+  MMR_ROWS_SHARED;
+  page_compact_list<ApplyGroup, kPageSegment>(x, st, w, prefix);
 }
 
 __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_fork_plan_kernel(PageState st, PageWork w, const int32_t* parents,
@@ -114,9 +127,9 @@ __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_fork_plan_kernel(Pa
   page_fork_plan(x, st, w, prefix, parents, children, n);
 }
 
-__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_compact_plan_kernel(PageState st, PageWork w) {
+__global__ __launch_bounds__(kPagePlanThreads) void mmr_page_compact_plan_kernel(PageState st, PageWork w, bool whole) {
   MMR_PLAN_SHARED;
-  page_compact_plan(x, st, w, prefix);
+  page_compact_plan(x, st, w, prefix, whole);
 }
 
 __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_count_kernel(PageState st, PageWork w) {
@@ -125,10 +138,21 @@ __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_count_kernel(PageSt
 }
 
 __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_copy_plan_kernel(PageState st, PageWork w, const int32_t* src,
-                                                                              const int32_t* dst, int32_t n) {
+                                                                              const int32_t* dst, int32_t n, bool sorted) {
   __shared__ __attribute__((aligned(16))) int32_t scan[kScanInts];
   PlanGroup x(scan);
-  page_copy_plan(x, st, w, src, dst, n);
+  page_copy_plan(x, st, w, src, dst, n, sorted);
+}
+
+template <bool ALIGNED>
+__global__ __launch_bounds__(kPageThreads) void mmr_page_copy_few_kernel(PageState st, PageWork w, PageMover mv, const int32_t* src,
+                                                                         const int32_t* dst, int32_t n) {
+  __shared__ __attribute__((aligned(16))) int32_t scan[2 * (kPageThreads / 64) + 2];
+  __shared__ int32_t pairs[2 * kFewPairs];
+  ApplyGroup x(scan);
+  if (!page_copy_few(x, st, w, pairs, src, dst, n)) return;
+  page_move_chunk<StreamMem, ALIGNED>(mv, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; },
+                                      static_cast<uint32_t>(n), blockIdx.x, threadIdx.x);
 }
 
 __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_free_kernel(PageState st, PageWork w, const int32_t* slots) {
@@ -137,7 +161,10 @@ __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_free_kernel(PageSta
   page_free(x, st, w, scan, slots);
 }
 
-// The first `row_blocks` workgroups write tables (KIND 1: fork, 2: compact; 0: none), the others move pages.
+// The first `row_blocks` workgroups write tables (KIND 1: fork, 2: compact; 0: none), the others move pages.  The page that
+// a fork copies is often the last one of several entries: its loads go through the caches (256 sequences forked from 16,
+// 402 MB written: 82 us; past the caches 131 us).  A copy or a compact reads every page once, past the caches (copy of
+// 805 MB 308 us, through them 311; compact 719 and 728).
 template <int KIND, bool ALIGNED>
 __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState st, PageWork w, PageMover mv,
                                                                       const int32_t* parents, const int32_t* children, int32_t n,
@@ -150,31 +177,46 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState 
     else page_compact_rows(x, st, w, blockIdx.x, row_blocks);
     return;
   }
-  const uint32_t items = static_cast<uint32_t>(w.header[kPageMoves]) * mv.n_buffers * mv.chunks;
+  const uint32_t moves = static_cast<uint32_t>(w.header[kPageMoves]), items = moves * mv.n_buffers * mv.chunks;
   const uint32_t step = gridDim.x - row_blocks;
-  for (uint32_t item = blockIdx.x - row_blocks; item < items; item += step)
-    page_move_chunk<StreamMem, ALIGNED>(mv, w.moves, item, threadIdx.x);
+  for (uint32_t at = blockIdx.x - row_blocks; at < (items + 511u) / 512u * 512u; at += step) {
+    const uint32_t item = chunk_index(at, 64);  // runs of 64 neighbours share an XCD
+    typedef DeviceMem<KIND != 1, true> M;
+    if (item < items) page_move_chunk<M, ALIGNED>(mv, [&](uint32_t i) { return w.moves[i]; }, moves, item, threadIdx.x);
+  }
 }
 
-template <class T, int VEC, bool INTERLEAVED>
+// STREAM: a launch that writes more than the caches keep for a reader writes past them (queries, keys and values of 18,001
+// tokens, 443 MB in all: 82.4 -> 79.3 us; the gradient of bf16 [4,32,2048,128] 23.9 -> 20.7 us); what a small one
+// writes, a decode step's queries and keys, stays for the kernel that reads it next.
+template <class T, int VEC, bool INTERLEAVED, bool STREAM>
 __global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(RotaryArgs a) {
-  __shared__ __attribute__((aligned(16))) int32_t scan[2 * (kRotaryThreads / 64) + 2];
-  Workgroup<kRotaryThreads> x(scan);
+  Workgroup<kRotaryThreads> x(nullptr);
   const RotaryJob& j = a.jobs[blockIdx.y];
   if (x.block >= j.blocks) return;  // uniform over the workgroup
-  rotary_block<CachedMem, T, VEC, INTERLEAVED>(x, a, j);
+  rotary_block<DeviceMem<false, STREAM>, T, VEC, INTERLEAVED>(x, a, j);
 }
 
-uint32_t segments(const PageWork& w) { return static_cast<uint32_t>(w.n_segments); }
+// The launch before a plan, where the pool is more than a plan scans itself.
+hipError_t launch_scan(const PageState& st, const PageWork& w, bool live, hipStream_t stream) {
+  if (w.n_segments <= kPlanScans) return hipSuccess;
+  hipLaunchKernelGGL(mmr_page_scan_kernel, dim3(static_cast<uint32_t>(w.n_segments)), dim3(kPagePlanThreads), 0, stream, st, w, live);
+  return hipGetLastError();
+}
 
 // Workgroups of a move: one per chunk up to this many, which then loop.
 constexpr uint64_t kMaxMoveBlocks = 1u << 18;
+
+// Up to so many pages the plan of a compact lists the moves itself, in at most 8 rounds.
+constexpr int32_t kCompactWhole = 16384;
+// Up to so many chunks a copy of few pairs is one launch, whose workgroups each check all pairs.
+constexpr uint64_t kFewChunks = 4096;
 
 template <int KIND>
 hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
                         const int32_t* children, int32_t n, uint32_t row_blocks, hipStream_t stream) {
   const uint64_t items = static_cast<uint64_t>(mv.max_moves) * mv.mover.n_buffers * mv.mover.chunks;
-  const uint32_t movers = static_cast<uint32_t>(items < kMaxMoveBlocks ? items : kMaxMoveBlocks);
+  const uint32_t movers = static_cast<uint32_t>(items < kMaxMoveBlocks ? (items + 511) / 512 * 512 : kMaxMoveBlocks);
   if (movers + row_blocks == 0) return hipSuccess;
   if (mv.aligned)
     hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, true>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
@@ -187,9 +229,21 @@ hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLa
 
 }  // namespace
 
+// Extend is one launch where no call of this size can give out more pages than its last workgroup writes in a few rounds;
+// else a second one follows, which does the writing if there is more (768 prompts of 128 pages each: 97 us by one
+// workgroup) and otherwise ends at once.
+constexpr int64_t kExtendWhole = 16384;
+
 hipError_t launch_page_extend(const PageState& st, const PageWork& w, const int32_t* slots, const int32_t* counts, int32_t n,
                               hipStream_t stream) {
-  hipLaunchKernelGGL(mmr_page_extend_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w, slots, counts, n);
+  const int64_t most = static_cast<int64_t>(n) * st.B;
+  const bool whole = (most < st.P ? most : st.P) <= kExtendWhole;
+  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+  hipLaunchKernelGGL(mmr_page_extend_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, slots, counts, n, whole);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (whole) return hipSuccess;
+  hipLaunchKernelGGL(mmr_page_extend_rows_kernel, dim3(static_cast<uint32_t>(n < 4096 ? n : 4096)), dim3(kPageThreads), 0, stream, st,
+                     w, slots, counts, n);
   return hipGetLastError();
 }
 
@@ -200,35 +254,57 @@ hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_
 
 hipError_t launch_page_fork(const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children, int32_t n,
                             const PageMoveLaunch& mv, hipStream_t stream) {
-  hipLaunchKernelGGL(mmr_page_fork_plan_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w, parents, children, n);
+  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+  hipLaunchKernelGGL(mmr_page_fork_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, parents, children, n);
   if (hipError_t e = hipGetLastError()) return e;
   return launch_apply<1>(st, w, mv, parents, children, n, static_cast<uint32_t>(n < 4096 ? n : 4096), stream);
 }
 
 hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream) {
-  hipLaunchKernelGGL(mmr_page_compact_plan_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w);
+  const bool whole = st.P <= kCompactWhole;
+  if (hipError_t e = launch_scan(st, w, true, stream)) return e;
+  hipLaunchKernelGGL(mmr_page_compact_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, whole);
   if (hipError_t e = hipGetLastError()) return e;
+  if (!whole) {
+    const uint32_t blocks = (mv.max_moves + kPageThreads - 1) / kPageThreads;
+    hipLaunchKernelGGL(mmr_page_compact_list_kernel, dim3(blocks < 1024 ? blocks : 1024), dim3(kPageThreads), 0, stream, st, w);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
   return launch_apply<2>(st, w, mv, nullptr, nullptr, 0, static_cast<uint32_t>(st.S < 4096 ? st.S : 4096), stream);
 }
 
 hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
                             const PageMoveLaunch& mv, hipStream_t stream) {
-  hipLaunchKernelGGL(mmr_page_copy_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, src, dst, n);
+  const uint64_t items = static_cast<uint64_t>(n) * mv.mover.n_buffers * mv.mover.chunks;
+  if (n <= kFewPairs && items <= kFewChunks) {
+    const dim3 grid(static_cast<uint32_t>(items));
+    if (mv.aligned) hipLaunchKernelGGL(mmr_page_copy_few_kernel<true>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
+    else hipLaunchKernelGGL(mmr_page_copy_few_kernel<false>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
+    return hipGetLastError();
+  }
+  const bool sorted = st.P / 8 <= n;
+  hipLaunchKernelGGL(mmr_page_copy_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, src, dst, n, sorted);
   if (hipError_t e = hipGetLastError()) return e;
   return launch_apply<0>(st, w, mv, nullptr, nullptr, 0, 0, stream);
 }
 
 hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream) {
-  hipLaunchKernelGGL(mmr_page_count_kernel, dim3(segments(w)), dim3(kPagePlanThreads), 0, stream, st, w);
+  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+  hipLaunchKernelGGL(mmr_page_count_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w);
   return hipGetLastError();
 }
 
-hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, hipStream_t stream) {
+hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, bool past_caches,
+                         hipStream_t stream) {
   uint32_t blocks = 0;
   for (int i = 0; i < n_jobs; ++i) blocks = args.jobs[i].blocks > blocks ? args.jobs[i].blocks : blocks;
   if (!blocks) return hipSuccess;
   const dim3 grid(blocks, static_cast<uint32_t>(n_jobs)), threads(kRotaryThreads);
-#define MMR_ROTARY(T, V, I) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I>), grid, threads, 0, stream, args)
+#define MMR_ROTARY(T, V, I)                                                                                     \
+  do {                                                                                                         \
+    if (past_caches) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, true>), grid, threads, 0, stream, args);   \
+    else hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, false>), grid, threads, 0, stream, args);              \
+  } while (0)
 #define MMR_ROTARY_TYPE(T, V)                                     \
   do {                                                            \
     if (vectors && interleaved) MMR_ROTARY(T, V, true);           \

@@ -9,13 +9,15 @@
 // gives out the pages and writes a list of page moves; the application, in a launch of its own, writes the tables and
 // carries the moves out in every pool.
 //
-// Finding the lowest free pages: workgroup i reads refs of the i-th segment of pages and writes the segment's free ids,
-// in order, and their count; the workgroup that arrives last sums the counts and looks the k-th free page up by a binary
-// search over them.  One launch, no workgroup ever waits for another.
+// Finding the lowest free pages: workgroup i of a scan reads refs of the i-th segment of pages and writes the segment's
+// free ids, in order, and their count; the plan, one workgroup, sums the counts and looks the k-th free page up by a
+// binary search over them.  A pool of few segments is scanned by the plan itself.  (All in one launch, the plan being
+// the part of the workgroup that arrives last, needs fences between the XCDs' caches, which cost more than a launch:
+// extend over 98 segments 50 us, over two 16 us and up to 54 us behind large copies, where one segment takes 6.)
 //
 // X is the workgroup: the GPU's (page_kernels.hip) or, in the tests, a set of host threads.  It has kThreads, tid,
 // block, blocks, sync(), scan(v, &total) (exclusive sum over the threads), any(flags) (bitwise or over the threads),
-// last_block(counter), atomic_add / atomic_exch / atomic_or.
+// atomic_add / atomic_exch / atomic_or.
 #ifndef MMR_CSRC_PAGE_OPS_H_
 #define MMR_CSRC_PAGE_OPS_H_
 
@@ -39,11 +41,12 @@ struct PageState {
   FastDiv div_T;
 };
 
-enum PageHeader { kPageCounter = 0, kPageOk = 1, kPageMoves = 2, kPageStatus = 3, kPageLive = 4, kPageHeaderInts = 64 };
+enum PageHeader { kPageOk = 1, kPageMoves = 2, kPageStatus = 3, kPageLive = 4, kPageFree = 5, kPageRows = 6, kPageHeaderInts = 64 };
 
 struct PageWork {
   int32_t* header;
-  int32_t* seg_free;  // free pages of every segment
+  int32_t* seg_free;    // free pages of every segment
+  int32_t* seg_before;  // free pages before every segment, once a plan has summed them
   int32_t* free_ids;  // segment s's free ids at s * segment size, ascending
   int32_t* live_ids;
   int32_t* mark;  // max(S, P) zeros between calls
@@ -55,6 +58,7 @@ struct PageWork {
 };
 
 constexpr int kPagesPerThread = 4;
+constexpr int32_t kExtendFew = 4096;  // fresh pages up to which the plan of extend writes the tables itself
 constexpr int32_t kMaxPageSegments = 4096;
 
 // One buffer of a pool: the tile of one device.
@@ -67,7 +71,7 @@ struct PageMover {
   const PageBuffer* buffers;
   uint32_t n_buffers;
   uint32_t chunks;  // chunks of kPageChunkBytes in the largest page
-  FastDiv div_chunks, div_buffers;
+  FastDiv div_chunks;
 };
 
 constexpr uint32_t kPageChunkBytes = 8192;
@@ -78,37 +82,52 @@ MMR_HD int32_t page_blocks(const PageState& st, int32_t tokens) {
   return full + (full * static_cast<int64_t>(st.T) != tokens);
 }
 
-// Free (and live) ids of this workgroup's segment.
+// Free (and live) ids of a segment.
 template <class X>
-MMR_HD void page_scan_segment(X& x, const PageState& st, const PageWork& w, bool live) {
+MMR_HD void page_scan_segment(X& x, const PageState& st, const PageWork& w, int32_t segment, bool live) {
   constexpr int32_t kSegment = kPagesPerThread * X::kThreads;
-  const int32_t at = static_cast<int32_t>(x.block) * kSegment + x.tid * kPagesPerThread;
+  const int32_t at = segment * kSegment + x.tid * kPagesPerThread;
   int32_t r[kPagesPerThread];
   x.load4(st.refs, at, st.P, r);  // ids beyond the pool read as in use
   int32_t n_free = 0;
   for (int i = 0; i < kPagesPerThread; ++i) n_free += r[i] == 0;
   int32_t total = 0;
   const int32_t before = x.scan(n_free, &total);
-  int32_t f = static_cast<int32_t>(x.block) * kSegment + before;
+  int32_t f = segment * kSegment + before;
   int32_t l = at - before;  // the segment's ids before this thread's that are not free
   for (int i = 0; i < kPagesPerThread; ++i) {
     if (at + i >= st.P) break;
     if (r[i] == 0) w.free_ids[f++] = at + i;
     else if (live) w.live_ids[l++] = at + i;
   }
-  if (x.tid == 0) w.seg_free[x.block] = total;
+  if (x.tid == 0) w.seg_free[segment] = total;
 }
 
-// The free pages of all segments, once every segment is scanned (last workgroup only).
+// Up to so many segments a plan scans itself.
+constexpr int32_t kPlanScans = 2;
+
 template <class X>
+MMR_HD void page_plan_scan(X& x, const PageState& st, const PageWork& w, bool live) {
+  if (w.n_segments > kPlanScans) return;  // done by the launch before
+  for (int32_t s = 0; s < w.n_segments; ++s) page_scan_segment(x, st, w, s, live);
+  x.sync();
+}
+
+// The free pages of all segments, once every segment is scanned: in the plan's last workgroup, or (`counted`) in a later
+// launch.
+template <class X, int32_t kSegment = kPagesPerThread * X::kThreads>
 struct FreePages {
-  static constexpr int32_t kSegment = kPagesPerThread * X::kThreads;
   const PageWork* w;
   int32_t* prefix;  // shared: free pages before every segment
   int32_t total;
-  int32_t P;
 
-  MMR_HD FreePages(X& x, const PageState& st, const PageWork& work, int32_t* shared) : w(&work), prefix(shared), total(0), P(st.P) {
+  MMR_HD FreePages(X& x, const PageWork& work, int32_t* shared, bool counted = false) : w(&work), prefix(shared), total(0) {
+    if (counted) {
+      for (int32_t s = x.tid; s < work.n_segments; s += X::kThreads) prefix[s] = work.seg_before[s];
+      total = work.header[kPageFree];
+      x.sync();
+      return;
+    }
     for (int32_t base = 0; base < work.n_segments; base += X::kThreads) {
       const int32_t s = base + x.tid;
       int32_t sum = 0;
@@ -117,6 +136,10 @@ struct FreePages {
       total += sum;
     }
     x.sync();
+  }
+  // for the launches behind a plan
+  MMR_HD void publish(X& x) const {
+    for (int32_t s = x.tid; s < w->n_segments; s += X::kThreads) w->seg_before[s] = prefix[s];
   }
   // last segment whose count of earlier pages is at most k
   template <class Before>
@@ -186,9 +209,8 @@ MMR_HD uint32_t page_fork_entry(X& x, const PageState& st, const PageWork& w, in
 template <class X>
 MMR_HD void page_fork_plan(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* parents,
                            const int32_t* children, int32_t n) {
-  page_scan_segment(x, st, w, false);
-  if (!x.last_block(&w.header[kPageCounter])) return;
-  const FreePages<X> pages(x, st, w, shared);
+  page_plan_scan(x, st, w, false);
+  const FreePages<X> pages(x, w, shared);
   int32_t fresh = 0;
   uint32_t bad = 0;
   for (int32_t base = 0; base < n; base += X::kThreads) {
@@ -241,12 +263,13 @@ MMR_HD void page_fork_rows(X& x, const PageState& st, const PageWork& w, const i
   if (bad) x.atomic_or(&w.header[kPageStatus], static_cast<int32_t>(bad));
 }
 
+// The plan writes the tables itself if that takes few rounds, or `whole` says that no launch follows; else page_extend_rows
+// does.
 template <class X>
-MMR_HD void page_extend(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* slots,
-                        const int32_t* counts, int32_t n) {
-  page_scan_segment(x, st, w, false);
-  if (!x.last_block(&w.header[kPageCounter])) return;
-  const FreePages<X> pages(x, st, w, shared);
+MMR_HD void page_extend_plan(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* slots,
+                             const int32_t* counts, int32_t n, bool whole) {
+  page_plan_scan(x, st, w, false);
+  const FreePages<X> pages(x, w, shared);
   int64_t fresh = 0;
   uint32_t bad = 0;
   for (int32_t base = 0; base < n; base += X::kThreads) {
@@ -285,7 +308,8 @@ MMR_HD void page_extend(X& x, const PageState& st, const PageWork& w, int32_t* s
   bad = x.any(bad);  // every mark is set and every rank written by now
   for (int32_t e = x.tid; e < n; e += X::kThreads)
     if (slots[e] >= 0 && slots[e] < st.S) x.atomic_exch(&w.mark[slots[e]], 0);
-  if (!bad) {
+  const bool rows = !bad && !whole && fresh > kExtendFew;
+  if (!bad && !rows) {
     for (int32_t k = x.tid; k < static_cast<int32_t>(fresh); k += X::kThreads) {
       int32_t lo = 0, hi = n;  // the last entry whose fresh pages start at or before k takes page k
       while (hi - lo > 1) {
@@ -299,7 +323,29 @@ MMR_HD void page_extend(X& x, const PageState& st, const PageWork& w, int32_t* s
     }
     for (int32_t e = x.tid; e < n; e += X::kThreads) st.lengths[slots[e]] = w.len[e] + counts[e];
   }
+  if (rows) pages.publish(x);
+  if (x.tid == 0) {
+    w.header[kPageFree] = pages.total;
+    w.header[kPageRows] = rows;
+  }
   page_verdict(x, w, bad, 0, -1);
+}
+
+template <class X, int32_t kSegment>
+MMR_HD void page_extend_rows(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* slots,
+                             const int32_t* counts, int32_t n) {
+  if (!w.header[kPageRows]) return;
+  const FreePages<X, kSegment> pages(x, w, shared, true);
+  for (int32_t e = static_cast<int32_t>(x.block); e < n; e += static_cast<int32_t>(x.blocks)) {
+    const int32_t old = w.len[e], all = old + counts[e], rank = w.rank[e], have = page_blocks(st, old);
+    int32_t* row = st.table + static_cast<int64_t>(slots[e]) * st.B + have;
+    for (int32_t i = x.tid, need = page_blocks(st, all) - have; i < need; i += X::kThreads) {
+      const int32_t page = pages.kth_free(rank + i);
+      row[i] = page;
+      st.refs[page] = 1;
+    }
+    if (x.tid == 0) st.lengths[slots[e]] = all;
+  }
 }
 
 // One workgroup per entry.  The length is taken by an exchange, so of two entries that name a sequence one frees it and
@@ -333,21 +379,40 @@ MMR_HD void page_free(X& x, const PageState& st, const PageWork& w, int32_t* sha
   if (bad) x.atomic_or(&w.header[kPageStatus], static_cast<int32_t>(bad));
 }
 
-template <class X>
-MMR_HD void page_compact_plan(X& x, const PageState& st, const PageWork& w, int32_t* shared) {
-  page_scan_segment(x, st, w, true);
-  if (!x.last_block(&w.header[kPageCounter])) return;
-  const FreePages<X> pages(x, st, w, shared);
-  const int32_t live = st.P - pages.total;
-  const int32_t moves = pages.free_below(live);  // as many live pages stand at or after `live`
-  for (int32_t k = x.tid; k < moves; k += X::kThreads) {
+// Moves k = first, first + step, ... of a compact.
+template <class Pages>
+MMR_HD void page_compact_moves(const PageState& st, const PageWork& w, const Pages& pages, int32_t moves, int32_t live,
+                               int32_t first, int32_t step) {
+  for (int32_t k = first; k < moves; k += step) {
     const int32_t dst = pages.kth_free(k), src = pages.kth_live(live - moves + k);
     w.moves[k] = PageMove{src, dst};
     w.map[src] = k;
     st.refs[dst] = st.refs[src];
     st.refs[src] = 0;
   }
+}
+
+// `whole`: the plan lists the moves itself; else page_compact_list does, in a launch of its own.
+template <class X>
+MMR_HD void page_compact_plan(X& x, const PageState& st, const PageWork& w, int32_t* shared, bool whole) {
+  page_plan_scan(x, st, w, true);
+  const FreePages<X> pages(x, w, shared);
+  const int32_t live = st.P - pages.total;
+  const int32_t moves = pages.free_below(live);  // as many live pages stand at or after `live`
+  if (whole) {
+    page_compact_moves(st, w, pages, moves, live, x.tid, X::kThreads);
+  } else {
+    pages.publish(x);
+    if (x.tid == 0) w.header[kPageFree] = pages.total;
+  }
   page_verdict(x, w, 0, moves, live);
+}
+
+template <class X, int32_t kSegment>
+MMR_HD void page_compact_list(X& x, const PageState& st, const PageWork& w, int32_t* shared) {
+  const FreePages<X, kSegment> pages(x, w, shared, true);
+  page_compact_moves(st, w, pages, w.header[kPageMoves], w.header[kPageLive], static_cast<int32_t>(x.block) * X::kThreads + x.tid,
+                     static_cast<int32_t>(x.blocks) * X::kThreads);
 }
 
 template <class X>
@@ -379,13 +444,16 @@ MMR_HD void page_compact_rows(X& x, const PageState& st, const PageWork& w, uint
 }
 
 // Pairs of a copy: every destination once, no destination that is also a source.  A page copied onto itself is no move.
+// `sorted`: the moves are listed by destination, which the marks give without a sort: a pass over the pages in place of
+// one over the pairs.
 template <class X>
-MMR_HD void page_copy_plan(X& x, const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n) {
+MMR_HD void page_copy_plan(X& x, const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
+                           bool sorted) {
   uint32_t bad = 0;
   for (int32_t e = x.tid; e < n; e += X::kThreads) {
     const int32_t s = src[e], d = dst[e];
     if (s < 0 || s >= st.P || d < 0 || d >= st.P) bad |= MMR_PAGES_BAD_PAGE;
-    else if (s != d && x.atomic_exch(&w.mark[d], 1)) bad |= MMR_PAGES_REPEATED;
+    else if (s != d && x.atomic_exch(&w.mark[d], e + 1)) bad |= MMR_PAGES_REPEATED;
   }
   x.sync();  // every mark is set
   int32_t moves = 0;
@@ -394,12 +462,26 @@ MMR_HD void page_copy_plan(X& x, const PageState& st, const PageWork& w, const i
     const int32_t s = e < n ? src[e] : 0, d = e < n ? dst[e] : 0;
     const bool inside = s >= 0 && s < st.P && d >= 0 && d < st.P;
     if (inside && s != d && w.mark[s]) bad |= MMR_PAGES_OVERLAP;
+    if (sorted) continue;
     int32_t sum = 0;
     const int32_t at = moves + x.scan(static_cast<int32_t>(inside && s != d), &sum);
     if (inside && s != d) w.moves[at] = PageMove{s, d};
     moves += sum;
   }
   bad = x.any(bad);  // every mark is read
+  for (int32_t base = 0; sorted && !bad && base < st.P; base += kPagesPerThread * X::kThreads) {
+    const int32_t first = base + x.tid * kPagesPerThread;
+    int32_t e[kPagesPerThread], here = 0, sum = 0;
+    for (int i = 0; i < kPagesPerThread; ++i) {
+      e[i] = first + i < st.P ? w.mark[first + i] : 0;
+      here += e[i] != 0;
+    }
+    int32_t at = moves + x.scan(here, &sum);
+    for (int i = 0; i < kPagesPerThread; ++i)
+      if (e[i]) w.moves[at++] = PageMove{src[e[i] - 1], first + i};
+    moves += sum;
+  }
+  x.sync();
   for (int32_t e = x.tid; e < n; e += X::kThreads) {
     const int32_t d = dst[e];
     if (d >= 0 && d < st.P) x.atomic_exch(&w.mark[d], 0);
@@ -407,25 +489,58 @@ MMR_HD void page_copy_plan(X& x, const PageState& st, const PageWork& w, const i
   page_verdict(x, w, bad, moves, -1);
 }
 
+constexpr int32_t kFewPairs = 64;
+
+// The same checks for at most kFewPairs pairs, made by every workgroup of the copy for itself, so that a small copy is one
+// launch: pair i is thread i's.  shared: 2 * kFewPairs words.  True if the pairs may be carried out.
+template <class X>
+MMR_HD bool page_copy_few(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* src, const int32_t* dst,
+                          int32_t n) {
+  int32_t s = -1, d = -1;
+  if (x.tid < n) {
+    s = src[x.tid], d = dst[x.tid];
+    shared[x.tid] = s;
+    shared[kFewPairs + x.tid] = d;
+  }
+  x.sync();
+  uint32_t bad = 0;
+  if (x.tid < n) {
+    if (s < 0 || s >= st.P || d < 0 || d >= st.P) {
+      bad |= MMR_PAGES_BAD_PAGE;
+    } else if (s != d) {
+      for (int32_t i = 0; i < n; ++i) {
+        if (i == x.tid || shared[i] == shared[kFewPairs + i]) continue;
+        if (shared[i] < 0 || shared[i] >= st.P) continue;  // a bad pair, as told by its own thread
+        if (shared[kFewPairs + i] == d) bad |= MMR_PAGES_REPEATED;
+        if (shared[kFewPairs + i] == s) bad |= MMR_PAGES_OVERLAP;
+      }
+    }
+  }
+  bad = x.any(bad);
+  if (bad && x.block == 0 && x.tid == 0) x.atomic_or(&w.header[kPageStatus], static_cast<int32_t>(bad));
+  return bad == 0;
+}
+
 // Pages in use, into header[kPageLive].
 template <class X>
 MMR_HD void page_count(X& x, const PageState& st, const PageWork& w, int32_t* shared) {
-  page_scan_segment(x, st, w, false);
-  if (!x.last_block(&w.header[kPageCounter])) return;
-  const FreePages<X> pages(x, st, w, shared);
+  page_plan_scan(x, st, w, false);
+  const FreePages<X> pages(x, w, shared);
   if (x.tid == 0) w.header[kPageLive] = st.P - pages.total;
 }
 
-// Chunk `item` of the moves: (move, buffer, chunk), the chunk fastest.  M: memory policy of chunk_ops.h.  Pages of a
-// multiple of 16 bytes move as aligned 16-byte vectors.  Others move as 16-byte vectors at any alignment, the last one
-// slid back to end with the page (it repeats bytes of its neighbour, with the same values), pages under 16 bytes byte by
-// byte.
-template <class M, bool ALIGNED>
-MMR_HD void page_move_chunk(const PageMover& m, const PageMove* moves, uint32_t item, uint32_t tid) {
+// Chunk `item` of the moves, buffer after buffer, move after move: the pages of one buffer are worked off together, so
+// that the workgroups in flight share their address translations.  move(i): move i.  M: memory policy of chunk_ops.h.
+// Pages of a multiple of 16 bytes move as aligned 16-byte vectors.  Others move as 16-byte vectors at any alignment, the
+// last one slid back to end with the page (it repeats bytes of its neighbour, with the same values), pages under 16 bytes
+// byte by byte.
+template <class M, bool ALIGNED, class Move>
+MMR_HD void page_move_chunk(const PageMover& m, Move move, uint32_t n_moves, uint32_t item, uint32_t tid) {
   const uint32_t rest = fdiv(item, m.div_chunks), chunk = item - rest * m.chunks;
-  const uint32_t mi = fdiv(rest, m.div_buffers), bi = rest - mi * m.n_buffers;
+  const uint32_t bi = rest / n_moves, mi = rest - bi * n_moves;
   const PageBuffer b = m.buffers[bi];
-  const PageMove mv = moves[mi];
+  const PageMove mv = move(mi);
+  if (mv.src == mv.dst) return;
   const uint64_t begin = static_cast<uint64_t>(chunk) * kPageChunkBytes;
   if (begin >= b.page_bytes) return;  // a smaller page than the largest
   const uint64_t left = b.page_bytes - begin;

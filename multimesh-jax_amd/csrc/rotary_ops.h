@@ -112,7 +112,7 @@ template <class T, int VEC>
 struct RotaryVec {
   static constexpr int kBytes = VEC * T::kBytes;
   static constexpr int kWords = (kBytes + 3) / 4;
-  uint32_t w[kWords];
+  uint32_t w[kWords] = {};
 
   template <class M>
   MMR_HD void load(typename M::cptr p) {
@@ -146,145 +146,166 @@ struct RotaryVec {
   MMR_HD void put1(float a) { w[0] = T::put(a); }  // VEC == 1
 };
 
-// Lane (row, unit) of workgroup `block` of a job.  A unit is two vectors (VEC pairs) of the rotated part, or one vector
-// of the rest.
+// Position and place of token t of a paged write: false if it has none (padding, or a bad entry: *bad).
+template <class X>
+MMR_HD bool rotary_place(X& x, const RotaryPages& pg, int32_t wave_token, int32_t t, int64_t* position, int32_t* page,
+                         int32_t* in_page, uint32_t* bad) {
+  // one token a sequence, without padding: entry t (a guess that a step of decoding always gets right saves it one load
+  // of the chain, and costs others nothing, as its loads wait for none)
+  int32_t entry = t < pg.n ? t : pg.n - 1;
+  if (!x.all(pg.begins[entry] <= t && t < pg.begins[entry + 1]))
+    entry = x.ended(pg.begins + 1, pg.n, wave_token);  // entries that end at or before the wave's first token
+  if (entry < pg.n && pg.begins[entry + 1] <= t) {     // a later token in a later entry
+    int32_t lo = entry + 1, hi = pg.n;
+    while (lo < hi) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (pg.begins[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    entry = lo;
+  }
+  if (entry >= pg.n) return false;  // behind the last sequence
+  const int32_t begin = pg.begins[entry], end = pg.begins[entry + 1], slot = pg.slots[entry];
+  if (t < begin) return false;  // before the first one
+  if (slot < 0 || slot >= pg.S) {
+    *bad = MMR_PAGES_BAD_SEQUENCE;
+    return false;
+  }
+  const int64_t p = static_cast<int64_t>(pg.lengths[slot]) - end + t;
+  if (p < 0 || p >= pg.capacity) {
+    *bad = MMR_PAGES_TOO_LONG;
+    return false;
+  }
+  const int32_t at = static_cast<int32_t>(fdiv(static_cast<uint32_t>(p), pg.div_T));
+  *position = p;
+  *in_page = static_cast<int32_t>(p) - at * pg.T;
+  *page = pg.table[static_cast<int64_t>(slot) * pg.B + at];
+  if (*page < 0 || *page >= pg.P) *bad = MMR_PAGES_BAD_PAGE;
+  return *bad == 0;
+}
+
+// Lane (row, unit) of workgroup `block` of a job.  A unit is what a lane turns: the two vectors that hold VEC pairs, or,
+// interleaved, one vector of VEC / 2 pairs; in the rest of the row it is one vector.  The rows are loaded before the
+// position is looked up: the look-up is a chain of four loads.
 template <class M, class T, int VEC, bool INTERLEAVED, class X>
 MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
   constexpr int kVecBytes = VEC * T::kBytes;
+  constexpr bool kTwo = T::kBytes > 1 && (!INTERLEAVED || VEC == 1);  // a unit of the rotated part is two vectors
+  constexpr int kPairs = INTERLEAVED && VEC > 1 ? VEC / 2 : VEC;      // and so many pairs
   const uint32_t group = fdiv(x.block, j.div_head_groups), hg = x.block - group * j.head_groups;
   const uint32_t row = fdiv(static_cast<uint32_t>(x.tid), j.div_lanes), lane = static_cast<uint32_t>(x.tid) - row * j.lanes;
   const uint32_t tsub = fdiv(row, j.div_head_lanes), hsub = row - tsub * j.head_lanes;
-  const uint32_t t0 = group * j.token_lanes, token = t0 + tsub;
-  bool on = tsub < j.token_lanes && token < j.tokens;
+  const uint32_t token = group * j.token_lanes + tsub;
+  const bool on = tsub < j.token_lanes && token < j.tokens;
+  const uint32_t outer = fdiv(on ? token : 0u, j.div_seq), seq = (on ? token : 0u) - outer * j.seq;
+  const char* const src = j.src + (static_cast<int64_t>(outer) * j.src_outer + static_cast<int64_t>(seq) * j.src_seq);
+  const uint32_t h0 = hg * j.head_lanes * j.head_steps + hsub;
 
-  int64_t position = 0;
-  const char* src = j.src;
-  char* dst = j.dst;
-  if (j.paged) {
-    // entry of the workgroup's first token: how many entries end at or before it (all threads, two barriers)
-    const RotaryPages& pg = a.pages;
-    int32_t ended = 0, entry = 0;
-    for (int32_t i = x.tid; i < pg.n; i += kRotaryThreads) ended += pg.begins[i + 1] <= static_cast<int32_t>(t0);
-    x.scan(ended, &entry);
-    if (!on) return;
-    const int32_t t = static_cast<int32_t>(token);
-    if (entry < pg.n && pg.begins[entry + 1] <= t) {  // a later token of the workgroup in a later entry
-      int32_t lo = entry + 1, hi = pg.n;
-      while (lo < hi) {
-        const int32_t mid = (lo + hi) >> 1;
-        if (pg.begins[mid + 1] <= t) lo = mid + 1;
-        else hi = mid;
-      }
-      entry = lo;
-    }
-    if (entry >= pg.n) return;  // behind the last sequence
-    const int32_t begin = pg.begins[entry], end = pg.begins[entry + 1], slot = pg.slots[entry];
-    if (t < begin) return;  // before the first one
-    uint32_t bad = 0;
-    int32_t page = 0, in_page = 0;
-    if (slot < 0 || slot >= pg.S) {
-      bad = MMR_PAGES_BAD_SEQUENCE;
-    } else {
-      const int64_t p = static_cast<int64_t>(pg.lengths[slot]) - (static_cast<int64_t>(end) - begin) + (static_cast<int64_t>(t) - begin);
-      if (p < 0 || p >= pg.capacity) {
-        bad = MMR_PAGES_TOO_LONG;
-      } else {
-        position = p;
-        const int32_t at = static_cast<int32_t>(fdiv(static_cast<uint32_t>(p), pg.div_T));
-        in_page = static_cast<int32_t>(p) - at * pg.T;
-        page = pg.table[static_cast<int64_t>(slot) * pg.B + at];
-        if (page < 0 || page >= pg.P) bad = MMR_PAGES_BAD_PAGE;
+  // byte offsets in a row of the two vectors of a unit (of the one, for units of the rest)
+  auto offsets = [&](uint32_t unit, int64_t* off_a, int64_t* off_b) {
+    if (!kTwo || unit >= j.rot_units)
+      *off_a = *off_b = static_cast<int64_t>(unit + (kTwo ? j.rot_units : 0)) * kVecBytes;
+    else if (INTERLEAVED) *off_a = static_cast<int64_t>(2) * unit * kVecBytes, *off_b = *off_a + kVecBytes;
+    else *off_a = static_cast<int64_t>(unit) * kVecBytes, *off_b = *off_a + static_cast<int64_t>(a.half) * T::kBytes;
+  };
+  RotaryVec<T, VEC> va[kRotaryHeads], vb[kRotaryHeads];
+  auto load = [&](uint32_t unit) {
+    int64_t off_a, off_b;
+    offsets(unit, &off_a, &off_b);
+#pragma unroll
+    for (uint32_t k = 0; k < kRotaryHeads; ++k) {
+      const uint32_t h = h0 + k * j.head_lanes;
+      if (k < j.head_steps && h < j.heads) {
+        va[k].template load<M>(M::cplace(src + (h * j.src_head + off_a)));
+        if (kTwo && unit < j.rot_units) vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
       }
     }
-    if (bad) {
-      if (lane == 0 && hsub == 0) x.atomic_or(pg.status, static_cast<int32_t>(bad));
-      return;
+  };
+  uint64_t f[kPairs];
+  auto load_frequencies = [&](uint32_t unit) {
+    if (T::kBytes > 1 && unit < j.rot_units) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) f[i] = a.frequency[unit * kPairs + i];
     }
-    src += static_cast<int64_t>(token) * j.src_seq;
-    if (j.paged == 1) dst += static_cast<int64_t>(page) * j.dst_outer + static_cast<int64_t>(in_page) * j.dst_seq;
-    else dst += static_cast<int64_t>(token) * j.dst_seq;  // queries: turned by the token's position, written beside it
-  } else {
-    if (!on) return;
-    const uint32_t outer = fdiv(token, j.div_seq), s = token - outer * j.seq;
-    position = j.positions ? j.positions[static_cast<int64_t>(outer) * j.pos_outer + static_cast<int64_t>(s) * j.pos_seq]
-                           : j.base + s;
-    src += static_cast<int64_t>(outer) * j.src_outer + static_cast<int64_t>(s) * j.src_seq;
-    dst += static_cast<int64_t>(outer) * j.dst_outer + static_cast<int64_t>(s) * j.dst_seq;
+  };
+  if (on) {
+    load(lane);
+    load_frequencies(lane);
   }
 
-  const uint32_t h0 = hg * j.head_lanes * j.head_steps + hsub;
-  for (uint32_t unit = lane; unit < j.units; unit += j.lanes) {
-    if (unit >= j.rot_units) {
-      const int64_t off = (2 * static_cast<int64_t>(j.rot_units) + (unit - j.rot_units)) * kVecBytes;
-      for (uint32_t i = 0; i < j.head_steps; i += kRotaryHeads) {
-        RotaryVec<T, VEC> v[kRotaryHeads];
-#pragma unroll
-        for (uint32_t k = 0; k < kRotaryHeads; ++k) {
-          const uint32_t h = h0 + (i + k) * j.head_lanes;
-          if (i + k < j.head_steps && h < j.heads) v[k].template load<M>(M::cplace(src + (h * j.src_head + off)));
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kRotaryHeads; ++k) {
-          const uint32_t h = h0 + (i + k) * j.head_lanes;
-          if (i + k < j.head_steps && h < j.heads) v[k].template store<M>(M::place(dst + (h * j.dst_head + off)));
-        }
-      }
-      continue;
+  int64_t position = 0;
+  char* dst = j.dst;
+  if (j.paged) {
+    // the token of the wave's first lane, for all lanes to look up together
+    const uint32_t first = fdiv(fdiv(static_cast<uint32_t>(x.tid) & ~63u, j.div_lanes), j.div_head_lanes);
+    const int32_t wave_token = static_cast<int32_t>(group * j.token_lanes + first);
+    int32_t page = 0, in_page = 0;
+    uint32_t bad = 0;
+    // lanes without a token ask for their wave's first one and go no further
+    const bool there = rotary_place(x, a.pages, wave_token, on ? static_cast<int32_t>(token) : wave_token, &position, &page, &in_page, &bad);
+    if (!on) return;
+    if (!there) {
+      if (bad && lane == 0 && hsub == 0) x.atomic_or(a.pages.status, static_cast<int32_t>(bad));
+      return;
     }
-    if constexpr (T::kBytes > 1) {
-      // byte offsets of the unit's two vectors and the pairs they hold
-      int64_t off_a, off_b;
-      if (INTERLEAVED && VEC == 1) off_a = static_cast<int64_t>(2) * unit * kVecBytes, off_b = off_a + kVecBytes;
-      else off_a = static_cast<int64_t>(unit) * kVecBytes, off_b = off_a + static_cast<int64_t>(a.half) * T::kBytes;
-      float s[VEC], c[VEC];
+    if (j.paged == 1) dst += static_cast<int64_t>(page) * j.dst_outer + static_cast<int64_t>(in_page) * j.dst_seq;
+    else dst += static_cast<int64_t>(seq) * j.dst_seq;  // queries: turned by the token's position, written beside it
+  } else {
+    if (!on) return;
+    position = j.positions ? j.positions[static_cast<int64_t>(outer) * j.pos_outer + static_cast<int64_t>(seq) * j.pos_seq]
+                           : j.base + seq;
+    dst += static_cast<int64_t>(outer) * j.dst_outer + static_cast<int64_t>(seq) * j.dst_seq;
+  }
+
+  for (uint32_t unit = lane;;) {
+    int64_t off_a, off_b;
+    offsets(unit, &off_a, &off_b);
+    if (T::kBytes > 1 && unit < j.rot_units) {
+      float s[kPairs], c[kPairs];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        uint32_t pair;
-        if (!INTERLEAVED || VEC == 1) pair = unit * VEC + i;
-        else pair = i < VEC / 2 ? unit * (VEC / 2) + i : (a.half + unit * VEC) / 2 + (i - VEC / 2);
-        turn_sincos(turns_at(position, a.frequency[pair]), &s[i], &c[i]);
+      for (int i = 0; i < kPairs; ++i) {
+        turn_sincos(turns_at(position, f[i]), &s[i], &c[i]);
         s[i] *= a.sine;
         c[i] *= a.magnitude;
       }
-      for (uint32_t i = 0; i < j.head_steps; i += kRotaryHeads) {
-        RotaryVec<T, VEC> va[kRotaryHeads], vb[kRotaryHeads];
 #pragma unroll
-        for (uint32_t k = 0; k < kRotaryHeads; ++k) {
-          const uint32_t h = h0 + (i + k) * j.head_lanes;
-          if (i + k < j.head_steps && h < j.heads) {
-            va[k].template load<M>(M::cplace(src + (h * j.src_head + off_a)));
-            vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
+      for (uint32_t k = 0; k < kRotaryHeads; ++k) {
+        if (k >= j.head_steps) break;  // uniform over the launch
+        if constexpr (VEC == 1) {
+          const float xa = va[k].get(0), xb = vb[k].get(0);
+          va[k].put1(xa * c[0] - xb * s[0]);
+          vb[k].put1(xb * c[0] + xa * s[0]);
+        } else if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const float xa = va[k].get(2 * i), xb = va[k].get(2 * i + 1);
+            va[k].put2(2 * i, xa * c[i] - xb * s[i], xb * c[i] + xa * s[i]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float a0 = va[k].get(e), a1 = va[k].get(e + 1), b0 = vb[k].get(e), b1 = vb[k].get(e + 1);
+            va[k].put2(e, a0 * c[e] - b0 * s[e], a1 * c[e + 1] - b1 * s[e + 1]);
+            vb[k].put2(e, b0 * c[e] + a0 * s[e], b1 * c[e + 1] + a1 * s[e + 1]);
           }
         }
-#pragma unroll
-        for (uint32_t k = 0; k < kRotaryHeads; ++k) {
-          const uint32_t h = h0 + (i + k) * j.head_lanes;
-          if (i + k >= j.head_steps || h >= j.heads) continue;
-          if constexpr (VEC == 1) {
-            const float xa = va[k].get(0), xb = vb[k].get(0);
-            va[k].put1(xa * c[0] - xb * s[0]);
-            vb[k].put1(xb * c[0] + xa * s[0]);
-          } else if constexpr (INTERLEAVED) {
-#pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-              const float a0 = va[k].get(e), b0 = va[k].get(e + 1), a1 = vb[k].get(e), b1 = vb[k].get(e + 1);
-              const float c0 = c[e / 2], s0 = s[e / 2], c1 = c[VEC / 2 + e / 2], s1 = s[VEC / 2 + e / 2];
-              va[k].put2(e, a0 * c0 - b0 * s0, b0 * c0 + a0 * s0);
-              vb[k].put2(e, a1 * c1 - b1 * s1, b1 * c1 + a1 * s1);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-              const float a0 = va[k].get(e), a1 = va[k].get(e + 1), b0 = vb[k].get(e), b1 = vb[k].get(e + 1);
-              va[k].put2(e, a0 * c[e] - b0 * s[e], a1 * c[e + 1] - b1 * s[e + 1]);
-              vb[k].put2(e, b0 * c[e] + a0 * s[e], b1 * c[e + 1] + a1 * s[e + 1]);
-            }
-          }
+        const uint32_t h = h0 + k * j.head_lanes;
+        if (h < j.heads) {
           va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
-          vb[k].template store<M>(M::place(dst + (h * j.dst_head + off_b)));
+          if (kTwo) vb[k].template store<M>(M::place(dst + (h * j.dst_head + off_b)));
         }
       }
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < kRotaryHeads; ++k) {
+        const uint32_t h = h0 + k * j.head_lanes;
+        if (k < j.head_steps && h < j.heads) va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
+      }
     }
+    unit += j.lanes;
+    if (unit >= j.units) break;
+    load(unit);
+    load_frequencies(unit);
   }
 }
 
@@ -301,8 +322,9 @@ inline uint64_t rotary_shape(RotaryJob* j, uint32_t rot_units, uint32_t rest_uni
   if (j->head_lanes > rows) j->head_lanes = rows;
   j->token_lanes = rows / j->head_lanes;
   if (spread && j->token_lanes > 1 && j->tokens < 1024) j->token_lanes = 1;
-  j->head_steps = (j->heads + j->head_lanes - 1) / j->head_lanes;
-  if (j->head_steps > want) j->head_steps = want;
+  const uint32_t steps = (j->heads + j->head_lanes - 1) / j->head_lanes;
+  const uint32_t groups = (steps + want - 1) / want;
+  j->head_steps = (steps + groups - 1) / groups;  // 5 heads go as 3 and 2, not as 4 and 1
   const uint32_t per = j->head_lanes * j->head_steps;
   j->head_groups = (j->heads + per - 1) / per;
   const uint64_t blocks = (static_cast<uint64_t>(j->tokens) + j->token_lanes - 1) / j->token_lanes * j->head_groups;

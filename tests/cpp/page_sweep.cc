@@ -66,13 +66,15 @@ struct Lanes {
     }
     return all;
   }
+  bool all(bool v) { return v; }  // a lane is a wave of its own here
+  int32_t ended(const int32_t* ends, int32_t n, int32_t t) {
+    int32_t count = 0;
+    while (count < n && ends[count] <= t) ++count;
+    return count;
+  }
   int32_t atomic_add(int32_t* p, int32_t v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
   int32_t atomic_exch(int32_t* p, int32_t v) { return __atomic_exchange_n(p, v, __ATOMIC_SEQ_CST); }
   void atomic_or(int32_t* p, int32_t v) { __atomic_fetch_or(p, v, __ATOMIC_SEQ_CST); }
-  bool last_block(int32_t*) {  // workgroups run one after the other
-    sync();
-    return block + 1 == blocks;
-  }
 };
 
 // `blocks` workgroups of K lanes, one after the other.
@@ -156,7 +158,7 @@ struct Cache {
   std::vector<uint64_t> page_bytes;
   Exact<int32_t> table, lengths, refs;
   std::vector<std::unique_ptr<Exact<char>>> pools;
-  Exact<int32_t> header, seg_free, free_ids, live_ids, mark, len, rank, map;
+  Exact<int32_t> header, seg_free, seg_before, free_ids, live_ids, mark, len, rank, map;
   Exact<PageMove> moves;
   Exact<PageBuffer> buffers;
   PageState st;
@@ -166,7 +168,7 @@ struct Cache {
 
   Cache(int32_t s, int32_t b, int32_t p, int32_t t, const std::vector<uint64_t>& bytes)
       : S(s), B(b), P(p), T(t), page_bytes(bytes), table(static_cast<size_t>(s) * b, 0x7b), lengths(s), refs(p), header(kPageHeaderInts),
-        seg_free(segs(p), 0x55), free_ids(segs(p) * kSegment, 0x55), live_ids(segs(p) * kSegment, 0x55), mark(std::max(s, p)),
+        seg_free(segs(p), 0x55), seg_before(segs(p), 0x55), free_ids(segs(p) * kSegment, 0x55), live_ids(segs(p) * kSegment, 0x55), mark(std::max(s, p)),
         len(s, 0x55), rank(s, 0x55), map(p, 0x55), moves(std::max(s, p), 0x55), buffers(bytes.size()) {
     uint64_t largest = 0;
     for (size_t i = 0; i < bytes.size(); ++i) {
@@ -178,8 +180,8 @@ struct Cache {
     const uint32_t chunks = static_cast<uint32_t>((largest + kPageChunkBytes - 1) / kPageChunkBytes);
     const int32_t capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(B) * T, 0x7fffffff));
     st = {table.p, lengths.p, refs.p, S, B, P, T, capacity, make_fastdiv(static_cast<uint32_t>(T))};
-    w = {header.p, seg_free.p, free_ids.p, live_ids.p, mark.p, len.p, rank.p, moves.p, map.p, segs(p)};
-    mover = {buffers.p, static_cast<uint32_t>(bytes.size()), chunks, make_fastdiv(chunks), make_fastdiv(static_cast<uint32_t>(bytes.size()))};
+    w = {header.p, seg_free.p, seg_before.p, free_ids.p, live_ids.p, mark.p, len.p, rank.p, moves.p, map.p, segs(p)};
+    mover = {buffers.p, static_cast<uint32_t>(bytes.size()), chunks, make_fastdiv(chunks)};
   }
   static int32_t segs(int32_t p) { return (p + kSegment - 1) / kSegment; }
 
@@ -206,6 +208,11 @@ struct Cache {
     header[kPageStatus] = 0;
     return s;
   }
+  template <class Move>
+  void chunk(uint32_t item, uint32_t n, uint32_t tid, Move m) {
+    if (aligned) page_move_chunk<Mem, true>(mover, m, n, item, tid);
+    else page_move_chunk<Mem, false>(mover, m, n, item, tid);
+  }
   void move(std::mt19937_64& rng) {
     if (!header[kPageOk]) return;
     const uint32_t items = static_cast<uint32_t>(header[kPageMoves]) * mover.n_buffers * mover.chunks;
@@ -213,8 +220,7 @@ struct Cache {
     for (uint32_t b = 0; b < blocks; ++b)
       for (uint32_t item = b; item < items; item += blocks)
         for (uint32_t tid = 0; tid < kPageThreads; ++tid)
-          if (aligned) page_move_chunk<Mem, true>(mover, moves.p, item, tid);
-          else page_move_chunk<Mem, false>(mover, moves.p, item, tid);
+          chunk(item, static_cast<uint32_t>(header[kPageMoves]), tid, [&](uint32_t i) { return moves[i]; });
   }
 };
 
@@ -358,12 +364,19 @@ uint32_t model_copy(const Cache& c, Model* m, const std::vector<int32_t>& s, con
   return 0;
 }
 
+void scan(const Cache& c, bool live) {
+  if (c.w.n_segments <= kPlanScans) return;
+  launch<K>(static_cast<uint32_t>(c.w.n_segments), [&](Lanes<K>& x) { page_scan_segment(x, c.st, c.w, static_cast<int32_t>(x.block), live); });
+}
+
 void cache_case(uint64_t seed) {
   std::mt19937_64 rng(seed);
   auto pick = [&](int32_t lo, int32_t hi) { return lo + static_cast<int32_t>(rng() % static_cast<uint64_t>(hi - lo + 1)); };
-  const int32_t T = pick(1, 3) == 1 ? 1 : pick(2, 9), S = pick(1, 40), B = pick(1, 12), P = pick(1, 260);
+  const int32_t T = pick(1, 3) == 1 ? 1 : pick(2, 9), S = pick(1, 40);
+  const bool big = pick(0, 11) == 0;  // enough pages for the second launch of extend to have work
+  const int32_t B = big ? 400 : pick(1, 12), P = big ? pick(5000, 9000) : pick(1, 260);
   std::vector<uint64_t> bytes;
-  const int kind = pick(0, 3);
+  const int kind = big ? 2 : pick(0, 3);
   for (int i = pick(1, 3); i > 0; --i)
     bytes.push_back(kind == 0 ? 16u * pick(1, 40) : kind == 1 ? 16u * pick(500, 600) : kind == 2 ? pick(1, 40) : pick(8190, 8300));
   Cache c(S, B, P, T, bytes);
@@ -389,7 +402,13 @@ void cache_case(uint64_t seed) {
       std::copy(a.begin(), a.end(), sa.p);
       std::copy(b.begin(), b.end(), sb.p);
       std::vector<int32_t> shared(kMaxPageSegments);
-      if (n) launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_extend(x, c.st, c.w, shared.data(), sa.p, sb.p, n); });
+      const bool whole = pick(0, 1);
+      if (n) {
+        scan(c, false);
+        launch<K>(1, [&](Lanes<K>& x) { page_extend_plan(x, c.st, c.w, shared.data(), sa.p, sb.p, n, whole); });
+        if (!whole)
+          launch<8>(3, [&](Lanes<8>& x) { page_extend_rows<Lanes<8>, kSegment>(x, c.st, c.w, shared.data(), sa.p, sb.p, n); });
+      }
       if (c.status() != want) die("extend: status", want, seed);
       c.check(m, "extend");
     } else if (op == 2) {
@@ -407,7 +426,8 @@ void cache_case(uint64_t seed) {
       std::copy(b.begin(), b.end(), sb.p);
       std::vector<int32_t> shared(kMaxPageSegments);
       if (n) {
-        launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_fork_plan(x, c.st, c.w, shared.data(), sa.p, sb.p, n); });
+        scan(c, false);
+        launch<K>(1, [&](Lanes<K>& x) { page_fork_plan(x, c.st, c.w, shared.data(), sa.p, sb.p, n); });
         if (c.header[kPageOk]) {
           const uint32_t rows = 1 + static_cast<uint32_t>(rng() % 4);
           launch<K>(rows, [&](Lanes<K>& x) { page_fork_rows(x, c.st, c.w, sa.p, sb.p, n, x.block, x.blocks); });
@@ -430,7 +450,10 @@ void cache_case(uint64_t seed) {
     } else if (pick(0, 1)) {
       model_compact(c, &m);
       std::vector<int32_t> shared(kMaxPageSegments);
-      launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_compact_plan(x, c.st, c.w, shared.data()); });
+      const bool whole = pick(0, 1);
+      scan(c, true);
+      launch<K>(1, [&](Lanes<K>& x) { page_compact_plan(x, c.st, c.w, shared.data(), whole); });
+      if (!whole) launch<8>(3, [&](Lanes<8>& x) { page_compact_list<Lanes<8>, kSegment>(x, c.st, c.w, shared.data()); });
       const uint32_t rows = 1 + static_cast<uint32_t>(rng() % 4);
       launch<K>(rows, [&](Lanes<K>& x) { page_compact_rows(x, c.st, c.w, x.block, x.blocks); });
       c.move(rng);
@@ -452,8 +475,22 @@ void cache_case(uint64_t seed) {
       Exact<int32_t> sa(a.size()), sb(b.size());
       std::copy(a.begin(), a.end(), sa.p);
       std::copy(b.begin(), b.end(), sb.p);
-      if (count) {
-        launch<K>(1, [&](Lanes<K>& x) { page_copy_plan(x, c.st, c.w, sa.p, sb.p, count); });
+      if (count && count <= kFewPairs && pick(0, 1)) {
+        int32_t pairs[2 * kFewPairs];
+        const uint32_t items = static_cast<uint32_t>(count) * c.mover.n_buffers * c.mover.chunks;
+        std::vector<char> ok(items);
+        launch<kFewPairs>(items, [&](Lanes<kFewPairs>& x) {
+          const bool go = page_copy_few(x, c.st, c.w, pairs, sa.p, sb.p, count);
+          if (x.tid == 0) ok[x.block] = go;
+          // by one thread: vectors that slide back repeat their neighbours' bytes, which the thread sanitizer takes for a race
+          for (uint32_t t = 0; go && x.tid == 0 && t < static_cast<uint32_t>(kPageThreads); ++t)
+            c.chunk(x.block, static_cast<uint32_t>(count), t, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; });
+        });
+        for (char g : ok)
+          if (g != ok[0]) die("workgroups disagree");
+      } else if (count) {
+        const bool sorted = pick(0, 1);
+        launch<K>(1, [&](Lanes<K>& x) { page_copy_plan(x, c.st, c.w, sa.p, sb.p, count, sorted); });
         c.move(rng);
       }
       if (c.status() != want) die("copy: status", want, seed);
@@ -461,7 +498,8 @@ void cache_case(uint64_t seed) {
     }
   }
   std::vector<int32_t> shared(kMaxPageSegments);
-  launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_count(x, c.st, c.w, shared.data()); });
+  scan(c, false);
+  launch<K>(1, [&](Lanes<K>& x) { page_count(x, c.st, c.w, shared.data()); });
   int32_t live = 0;
   for (int32_t i = 0; i < P; ++i) live += c.refs[i] != 0;
   if (c.header[kPageLive] != live) die("count", live, c.header[kPageLive]);
@@ -478,10 +516,13 @@ void corrupt_case(uint64_t seed) {
   std::vector<int32_t> shared(kMaxPageSegments);
   Exact<int32_t> a(S), b(S);
   for (int32_t s = 0; s < S; ++s) a[s] = s, b[s] = (s + 1) % S;
-  launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_extend(x, c.st, c.w, shared.data(), a.p, b.p, S); });
-  launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_fork_plan(x, c.st, c.w, shared.data(), a.p, b.p, S); });
+  scan(c, false);
+        launch<K>(1, [&](Lanes<K>& x) { page_extend_plan(x, c.st, c.w, shared.data(), a.p, b.p, S, true); });
+  scan(c, false);
+        launch<K>(1, [&](Lanes<K>& x) { page_fork_plan(x, c.st, c.w, shared.data(), a.p, b.p, S); });
   if (c.header[kPageOk]) die("a corrupt fork is taken");
-  launch<K>(c.w.n_segments, [&](Lanes<K>& x) { page_compact_plan(x, c.st, c.w, shared.data()); });
+  scan(c, true);
+      launch<K>(1, [&](Lanes<K>& x) { page_compact_plan(x, c.st, c.w, shared.data(), true); });
   launch<K>(3, [&](Lanes<K>& x) { page_compact_rows(x, c.st, c.w, x.block, x.blocks); });
   c.move(rng);
   launch<K>(S, [&](Lanes<K>& x) { page_free(x, c.st, c.w, shared.data(), a.p); });
@@ -502,7 +543,8 @@ void rotary_case(uint64_t seed, double eps) {
   std::mt19937_64 rng(seed);
   auto pick = [&](int32_t lo, int32_t hi) { return lo + static_cast<int32_t>(rng() % static_cast<uint64_t>(hi - lo + 1)); };
   const int unit = VEC == 1 ? 1 : 16 / T::kBytes;
-  const int half = unit * pick(1, VEC == 1 ? 9 : 3), dim = 2 * half + unit * pick(0, 3);
+  const int half = (INTERLEAVED && VEC > 1 ? unit / 2 : unit) * pick(1, VEC == 1 ? 9 : 3);
+  const int dim = 2 * half + unit * pick(0, 3);
   const int outer = pick(1, 2), seq = pick(1, 40), heads = pick(1, 11), paged = pick(0, 2);
   const bool in_place = paged != 1 && pick(0, 2) == 0, turn = !(paged && pick(0, 3) == 0), spread = pick(0, 1);
   const bool heads_minor = paged || pick(0, 1);
@@ -588,7 +630,7 @@ void rotary_case(uint64_t seed, double eps) {
   }
   const auto before = x.copy();
   const bool same = j.dst == x.p;
-  const int rot = turn ? half / VEC : 0, rest = turn ? (same ? 0 : (dim - 2 * half) / VEC) : dim / VEC;
+  const int rot = turn ? (INTERLEAVED && VEC > 1 ? 2 * half : half) / VEC : 0, rest = turn ? (same ? 0 : (dim - 2 * half) / VEC) : dim / VEC;
   rotary_shape(&j, rot, rest, j.src_head <= j.src_seq, spread);
   const RotaryArgs args = a;
   launch<kRotaryThreads>(j.blocks, [&](Lanes<kRotaryThreads>& l) { rotary_block<Mem, T, VEC, INTERLEAVED>(l, args, args.jobs[0]); });
