@@ -338,12 +338,12 @@ def _is_int32(dtype) -> bool:
     return known
 
 
-def _ids(a, what: str) -> Tuple[int, int]:
-    """(device address, entries) of an int32 array in device memory: a StoreHandle (S32, one device, rank 1), an array
-    object of a GPU framework (int32, contiguous, on the GPU), or such a pair itself."""
+def _ids(ctx: "ReshardContext", a, what: str) -> Tuple[int, int]:
+    """(device address, entries) of an int32 array in the memory of the context's GPU: a StoreHandle (S32, one device,
+    rank 1), an array object of a GPU framework (int32, contiguous), or such a pair itself."""
     if hasattr(a, "data_ptr"):
-        if not getattr(a, "is_cuda", False):
-            raise ValueError("%s: the array is not in device memory" % what)
+        if not getattr(a, "is_cuda", False) or a.get_device() != ctx.hip_device:
+            raise ValueError("%s: the array is not in the memory of GPU %d" % (what, ctx.hip_device))
         if not _is_int32(a.dtype) or not a.is_contiguous():
             raise ValueError("%s: ids are int32 and contiguous, not %s" % (what, a.dtype))
         return a.data_ptr(), a.numel()
@@ -351,7 +351,9 @@ def _ids(a, what: str) -> Tuple[int, int]:
         s = a.shape
         if s.dtype != B.DTYPES["S32"] or s.dev_count != 1 or s.ndims != 1:
             raise ValueError("%s: a store of ids is S32, of rank 1 and on one device" % what)
-        return a._ctx.SliceLocalShard(s.dev_start, a, wait=False), int(s.dims[0].size)
+        if a._ctx is not ctx:
+            raise ValueError("%s: the store belongs to another context" % what)
+        return ctx.SliceLocalShard(s.dev_start, a, wait=False), int(s.dims[0].size)
     if isinstance(a, tuple) and len(a) == 2:
         return int(a[0]), int(a[1])
     raise TypeError("%s: ids are a StoreHandle, an int32 array in device memory, or (device address, entries)" % what)
@@ -377,7 +379,7 @@ class PageCache:
         self._ctx, self._h, self._lib = ctx, handle, ctx._lib
 
     def _pairs(self, fn, a, b, what):
-        (pa, na), (pb, nb) = _ids(a, what[0]), _ids(b, what[1])
+        (pa, na), (pb, nb) = _ids(self._ctx, a, what[0]), _ids(self._ctx, b, what[1])
         if na != nb:
             raise ValueError("%d %s, %d %s" % (na, what[0], nb, what[1]))
         B.check(fn(self._h, pa, pb, na))
@@ -389,7 +391,7 @@ class PageCache:
         self._pairs(self._lib.mmr_pages_fork, parents, children, ("parents", "children"))
 
     def Free(self, sequences) -> None:
-        p, n = _ids(sequences, "sequences")
+        p, n = _ids(self._ctx, sequences, "sequences")
         B.check(self._lib.mmr_pages_free(self._h, p, n))
 
     def Copy(self, sources, destinations) -> None:
@@ -401,7 +403,7 @@ class PageCache:
     def Write(self, sequences, begins, k_pool: int, k: StoreHandle, v_pool: int = -1, v: Optional[StoreHandle] = None,
               rotary: Optional[RotaryPlan] = None, q: Optional[StoreHandle] = None, q_out: Optional[StoreHandle] = None) -> None:
         """New tokens into the pages (mmr_pages_write); `begins` has an entry more than `sequences`."""
-        (ps, n), (pb, nb) = _ids(sequences, "sequences"), _ids(begins, "begins")
+        (ps, n), (pb, nb) = _ids(self._ctx, sequences, "sequences"), _ids(self._ctx, begins, "begins")
         if nb != n + 1:
             raise ValueError("%d begins for %d sequences" % (nb, n))
         h = lambda s: s._h if s is not None else None  # noqa: E731
@@ -430,6 +432,7 @@ class ReshardContext:
     def __init__(self, hip_device: int = 0, hip_stream: Optional[int] = None):
         self._lib = B.load()
         self._h = C.c_void_p()
+        self.hip_device = hip_device
         B.check(self._lib.mmr_context_create(hip_device, C.c_void_p(hip_stream) if hip_stream else None,
                                              C.byref(self._h)))
 

@@ -4,6 +4,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
+#include <new>
+#include <set>
 #include <vector>
 
 #include "context_access.h"
@@ -72,6 +75,19 @@ int check_table(mmr_context* ctx, const mmr_store* s, int rank, const char* what
     if (d.size[i] < 1 || d.size[i] > 0x7fffffff)
       return fail(MMR_INVALID_ARGUMENT, "%s store has extent %lld along dim %d", what, (long long)d.size[i], i);
   return MMR_OK;
+}
+
+// No C++ exception leaves a C entry point (what can throw here is host memory running out).
+int exception_status() {
+  try {
+    throw;
+  } catch (const std::bad_alloc&) {
+    return fail(MMR_OUT_OF_MEMORY, "out of host memory");
+  } catch (const std::exception& e) {
+    return fail(MMR_INTERNAL, "%s", e.what());
+  } catch (...) {
+    return fail(MMR_INTERNAL, "unknown exception");
+  }
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -169,57 +185,50 @@ bool vector_rows(int64_t rotated, bool interleaved, int64_t dim, int itemsize) {
 
 constexpr uint64_t kMaxRotaryBlocks = (1u << 24) - 1;  // a grid has fewer than 2^32 threads
 
-struct RotaryLaunch {
-  mmr::RotaryArgs args{};
-  std::vector<mmr::RotaryJob> jobs;
-  int type = -1;
-  bool vectors = false, interleaved = false;
-  int64_t bytes = 0;  // written
-};
-
 constexpr int64_t kL2Bytes = int64_t{32} << 20;  // eight XCDs of 4 MiB
 
-void set_plan(RotaryLaunch* l, const mmr_rotary* r, bool backward) {
+void set_plan(mmr::RotaryLaunch* l, const mmr_rotary* r, bool backward) {
   if (!r) return;
-  l->args.frequency = reinterpret_cast<const uint64_t*>(r->block);
-  l->args.magnitude = r->magnitude;
-  l->args.sine = backward ? -r->magnitude : r->magnitude;
-  l->args.half = static_cast<uint32_t>(r->dim / 2);
+  l->angles = {reinterpret_cast<const uint64_t*>(r->block), r->magnitude, backward ? -r->magnitude : r->magnitude,
+               static_cast<uint32_t>(r->dim / 2)};
   l->interleaved = r->interleaved;
 }
 
-// Units of the jobs.  A launch of few rows takes one head a lane, so that its latency is one row's and not four.
-int shape_jobs(RotaryLaunch* l, const std::vector<int64_t>& dims, const std::vector<int>& turned, int itemsize) {
+// What of a row a launch does: its length in elements, and whether it is turned and in place (then the rest of it stays).
+struct Row {
+  int64_t dim;
+  bool turned, in_place;
+};
+
+// Units of the shapes, and the launches.  A call of few rows takes one head a lane, so that its latency is one row's and
+// not four.
+int launch_rows(mmr_context* ctx, mmr::RotaryLaunch* l, const std::vector<Row>& rows, int itemsize) {
   const int64_t vec = l->type < 0 ? (l->vectors ? 16 : 1) : (l->vectors ? 16 / itemsize : 1);
   const int64_t per = l->type < 0 ? itemsize : 1;  // raw rows are counted in bytes
-  int64_t lanes = 0;
+  int64_t lanes = 0, bytes = 0;
   std::vector<std::pair<uint32_t, uint32_t>> units;
-  for (size_t i = 0; i < l->jobs.size(); ++i) {
-    const int64_t rot = turned[i] ? static_cast<int64_t>(l->args.half) : 0;
-    const int64_t rest = turned[i] == 2 ? 0 : dims[i] * per - 2 * rot;  // 2: in place, what is not turned stays
+  for (const Row& r : rows) {
+    const int64_t rot = r.turned ? static_cast<int64_t>(l->angles.half) : 0;
+    const int64_t rest = r.in_place ? 0 : r.dim * per - 2 * rot;
     const bool one = l->interleaved && l->vectors;  // a unit is one vector, not two
     units.push_back({static_cast<uint32_t>((one ? 2 * rot : rot) / vec), static_cast<uint32_t>(rest / vec)});
-    const int64_t rows = static_cast<int64_t>(l->jobs[i].tokens) * l->jobs[i].heads;
-    lanes += rows * (units[i].first + units[i].second);
-    l->bytes += rows * dims[i] * itemsize;
+  }
+  for (const mmr::RotaryBuffer& b : l->buffers) {
+    const int64_t n = static_cast<int64_t>(b.outer) * b.seq * b.heads;
+    lanes += n * (units[b.shape].first + units[b.shape].second);
+    bytes += n * rows[b.shape].dim * itemsize;
   }
   const bool spread = lanes < 256 * 1024;  // a lane each would leave the 256 CUs under four workgroups
-  for (size_t i = 0; i < l->jobs.size(); ++i) {
-    mmr::RotaryJob& j = l->jobs[i];
+  for (size_t i = 0; i < l->shapes.size(); ++i) {
+    mmr::RotaryShape& j = l->shapes[i];
     if (mmr::rotary_shape(&j, units[i].first, units[i].second, j.src_head <= j.src_seq, spread) > kMaxRotaryBlocks)
-      return fail(MMR_UNSUPPORTED, "a tile of %u rows of %u heads is more than a launch takes", j.tokens, j.heads);
+      return fail(MMR_UNSUPPORTED, "a tile of %u tokens of %u heads is more than a launch takes", j.tokens, j.heads);
   }
-  return MMR_OK;
-}
-
-int launch_jobs(mmr_context* ctx, RotaryLaunch* l) {
-  for (size_t at = 0; at < l->jobs.size(); at += mmr::kRotaryMaxJobs) {
-    const int n = static_cast<int>(std::min<size_t>(mmr::kRotaryMaxJobs, l->jobs.size() - at));
-    std::copy(l->jobs.begin() + at, l->jobs.begin() + at + n, l->args.jobs);
-    MMR_HIP(mmr::launch_rotary(l->args, n, l->type, l->vectors, l->interleaved, l->bytes > kL2Bytes,
-                               mmr::context_stream(ctx)));
-    mmr::context_count(ctx, 1);
-  }
+  l->past_caches = bytes > kL2Bytes;
+  int launches = 0;
+  const hipError_t e = mmr::launch_rotary(*l, &launches, mmr::context_stream(ctx));
+  mmr::context_count(ctx, launches);
+  MMR_HIP(e);
   return MMR_OK;
 }
 
@@ -228,7 +237,7 @@ int launch_jobs(mmr_context* ctx, RotaryLaunch* l) {
 extern "C" {
 
 int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools, mmr_store* table, mmr_store* lengths,
-                     mmr_store* refs, int32_t page_tokens, mmr_pages** out) {
+                     mmr_store* refs, int32_t page_tokens, mmr_pages** out) try {
   if (!ctx || !out || (n_pools > 0 && !pools)) return fail(MMR_INVALID_ARGUMENT, "null argument");
   *out = nullptr;
   mmr::ContextLock lock(ctx);
@@ -250,12 +259,12 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
   auto p = std::make_unique<mmr_pages>();
   int64_t buffers = 0, largest = 0;
   bool aligned = true;
+  std::set<const mmr_store*> seen;
   for (int32_t i = 0; i < n_pools; ++i) {
     if (int rc = mmr::context_check_store(ctx, pools[i], "pool")) return rc;
     if (pools[i] == table || pools[i] == lengths || pools[i] == refs)
       return fail(MMR_INVALID_ARGUMENT, "pool %d is one of the tables", i);
-    for (int32_t j = 0; j < i; ++j)
-      if (pools[j] == pools[i]) return fail(MMR_INVALID_ARGUMENT, "pools %d and %d are the same store", j, i);
+    if (!seen.insert(pools[i]).second) return fail(MMR_INVALID_ARGUMENT, "pool %d is the same store as an earlier one", i);
     const Side& s = mmr::store_side(pools[i]);
     if (s.rank < 1 || s.size[0] != P || s.tiles[0] != 1)
       return fail(MMR_INVALID_ARGUMENT, "dim 0 of pool %d is not the %lld pages, unsharded", i, (long long)P);
@@ -300,20 +309,25 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
   p->move.aligned = aligned;
   p->table_id = mmr_store_id(table), p->lengths_id = mmr_store_id(lengths), p->refs_id = mmr_store_id(refs);
   p->epoch = mmr::context_store_epoch(ctx);
-  *out = p.get();
+  mmr_pages* handle = p.get();
   mmr::context_attach(ctx, std::move(p));
+  *out = handle;
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_destroy(mmr_pages* pages) {
+int mmr_pages_destroy(mmr_pages* pages) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr_context* ctx = pages->owner;
   mmr::ContextLock lock(ctx);
   mmr::context_detach(ctx, pages);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_extend(mmr_pages* pages, const int32_t* sequences, const int32_t* tokens, int32_t n) {
+int mmr_pages_extend(mmr_pages* pages, const int32_t* sequences, const int32_t* tokens, int32_t n) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, n, pages->state.S, "the sequences of the table")) return rc;
@@ -324,9 +338,11 @@ int mmr_pages_extend(mmr_pages* pages, const int32_t* sequences, const int32_t* 
   MMR_HIP(mmr::launch_page_extend(pages->state, pages->work, sequences, tokens, n, mmr::context_stream(pages->owner)));
   mmr::context_count(pages->owner, 1);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_free(mmr_pages* pages, const int32_t* sequences, int32_t n) {
+int mmr_pages_free(mmr_pages* pages, const int32_t* sequences, int32_t n) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, n, pages->state.S, "the sequences of the table")) return rc;
@@ -336,9 +352,11 @@ int mmr_pages_free(mmr_pages* pages, const int32_t* sequences, int32_t n) {
   MMR_HIP(mmr::launch_page_free(pages->state, pages->work, sequences, n, mmr::context_stream(pages->owner)));
   mmr::context_count(pages->owner, 1);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_fork(mmr_pages* pages, const int32_t* parents, const int32_t* children, int32_t n) {
+int mmr_pages_fork(mmr_pages* pages, const int32_t* parents, const int32_t* children, int32_t n) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, n, pages->state.S, "the sequences of the table")) return rc;
@@ -350,9 +368,11 @@ int mmr_pages_fork(mmr_pages* pages, const int32_t* parents, const int32_t* chil
                                 mmr::context_stream(pages->owner)));
   mmr::context_count(pages->owner, 2);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_compact(mmr_pages* pages) {
+int mmr_pages_compact(mmr_pages* pages) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, 0, 0, "")) return rc;
@@ -361,9 +381,11 @@ int mmr_pages_compact(mmr_pages* pages) {
                                    mmr::context_stream(pages->owner)));
   mmr::context_count(pages->owner, 2);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_copy(mmr_pages* pages, const int32_t* sources, const int32_t* destinations, int32_t n) {
+int mmr_pages_copy(mmr_pages* pages, const int32_t* sources, const int32_t* destinations, int32_t n) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, n, pages->state.P, "the pages of the pools")) return rc;
@@ -375,9 +397,11 @@ int mmr_pages_copy(mmr_pages* pages, const int32_t* sources, const int32_t* dest
                                 mmr::context_stream(pages->owner)));
   mmr::context_count(pages->owner, 2);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_pages_status(mmr_pages* pages, uint32_t* flags, int64_t* pages_in_use) {
+int mmr_pages_status(mmr_pages* pages, uint32_t* flags, int64_t* pages_in_use) try {
   if (!pages || !flags) return fail(MMR_INVALID_ARGUMENT, "null argument");
   mmr_context* ctx = pages->owner;
   mmr::ContextLock lock(ctx);
@@ -393,9 +417,11 @@ int mmr_pages_status(mmr_pages* pages, uint32_t* flags, int64_t* pages_in_use) {
   *flags = static_cast<uint32_t>(header[mmr::kPageStatus]);
   if (pages_in_use) *pages_in_use = header[mmr::kPageLive];
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* o, mmr_rotary** out) {
+int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* o, mmr_rotary** out) try {
   if (!ctx || !o || !out) return fail(MMR_INVALID_ARGUMENT, "null argument");
   *out = nullptr;
   mmr::ContextLock lock(ctx);
@@ -438,21 +464,26 @@ int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* o, mmr_rotary*
   r->magnitude = static_cast<float>(o->magnitude);
   if (int rc = mmr::context_take_block(ctx, turns.size() * 8, &r->block, &r->capacity)) return rc;
   if (int rc = mmr::context_upload(ctx, r->block, turns.data(), turns.size() * 8)) return rc;
-  *out = r.get();
+  mmr_rotary* handle = r.get();
   mmr::context_attach(ctx, std::move(r));
+  *out = handle;
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
-int mmr_rotary_destroy(mmr_rotary* rotary) {
+int mmr_rotary_destroy(mmr_rotary* rotary) try {
   if (!rotary) return fail(MMR_INVALID_ARGUMENT, "null rotary plan");
   mmr_context* ctx = rotary->owner;
   mmr::ContextLock lock(ctx);
   mmr::context_detach(ctx, rotary);
   return MMR_OK;
+} catch (...) {
+  return exception_status();
 }
 
 int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t seq_dim, mmr_store* positions, int64_t offset,
-                     uint32_t flags) {
+                     uint32_t flags) try {
   if (!rotary) return fail(MMR_INVALID_ARGUMENT, "null rotary plan");
   mmr_context* ctx = rotary->owner;
   mmr::ContextLock lock(ctx);
@@ -492,54 +523,61 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
     if (ps->size[ps->rank - 1] != s.size[seq_dim])
       return fail(MMR_INVALID_ARGUMENT, "positions of %lld, sequence of %lld", (long long)ps->size[ps->rank - 1], (long long)s.size[seq_dim]);
   }
-  RotaryLaunch l;
+  mmr::RotaryLaunch l;
   set_plan(&l, rotary, flags & MMR_ROTARY_BACKWARD);
   l.type = s.dtype;
   l.vectors = vector_rows(rotary->dim, rotary->interleaved, s.size[s.rank - 1], s.itemsize);
-  std::vector<int64_t> dims;
-  std::vector<int> turned;
+  const int64_t all_outer = outer >= 0 ? s.ext[outer] : 1, all_heads = head >= 0 ? s.ext[head] : 1, all_seq = s.ext[seq_dim];
+  if (all_outer == 0 || all_heads == 0 || all_seq == 0) return MMR_OK;  // an empty array
+  if (all_outer > 0x7fffffff / all_seq || all_heads > 0x7fffffff) return fail(MMR_UNSUPPORTED, "a tile of more than 2^31 rows");
+  mmr::RotaryShape shape{};
+  shape.tokens = static_cast<uint32_t>(all_outer * all_seq), shape.seq = static_cast<uint32_t>(all_seq);
+  shape.heads = static_cast<uint32_t>(all_heads);
+  shape.src_seq = shape.dst_seq = s.stride[seq_dim] * s.itemsize;
+  shape.src_outer = shape.dst_outer = outer >= 0 ? s.stride[outer] * s.itemsize : 0;
+  shape.src_head = shape.dst_head = head >= 0 ? s.stride[head] * s.itemsize : 0;
+  if (ps) {
+    shape.pos_seq = ps->stride[ps->rank - 1];
+    shape.pos_outer = ps->rank == 2 ? ps->stride[0] : 0;
+  }
+  l.shapes.push_back(shape);
+  bool in_place = true;
   for (int64_t k = 0; k < s.dev_count; ++k) {
-    mmr::RotaryJob j{};
-    j.src = mmr::store_tile(x, k);
-    j.dst = mmr::store_tile(out, k);
-    const int64_t n_outer = outer >= 0 ? tile_valid(s, k, outer) : 1, n_head = head >= 0 ? tile_valid(s, k, head) : 1;
-    const int64_t n_seq = tile_valid(s, k, seq_dim);
-    if (n_outer == 0 || n_head == 0 || n_seq == 0) continue;  // a tile of padding
-    if (n_outer * n_seq > 0x7fffffff || n_head > 0x7fffffff) return fail(MMR_UNSUPPORTED, "a tile of more than 2^31 rows");
-    j.tokens = static_cast<uint32_t>(n_outer * n_seq), j.seq = static_cast<uint32_t>(n_seq), j.heads = static_cast<uint32_t>(n_head);
-    j.src_seq = j.dst_seq = s.stride[seq_dim] * s.itemsize;
-    j.src_outer = j.dst_outer = outer >= 0 ? s.stride[outer] * s.itemsize : 0;
-    j.src_head = j.dst_head = head >= 0 ? s.stride[head] * s.itemsize : 0;
-    j.base = offset + tile_start(s, k, seq_dim);
+    mmr::RotaryBuffer b{};
+    b.src = mmr::store_tile(x, k);
+    b.dst = mmr::store_tile(out, k);
+    b.outer = static_cast<uint32_t>(outer >= 0 ? tile_valid(s, k, outer) : 1);
+    b.heads = static_cast<uint32_t>(head >= 0 ? tile_valid(s, k, head) : 1);
+    b.seq = static_cast<uint32_t>(tile_valid(s, k, seq_dim));
+    if (b.outer == 0 || b.heads == 0 || b.seq == 0) continue;  // a tile of padding
+    b.base = offset + tile_start(s, k, seq_dim);
     if (ps) {
       const int q = ps->rank - 1;
       // this device's positions cover its part of the sequence (and of dim 0)
       const int64_t at = tile_start(s, k, seq_dim) - tile_start(*ps, k, q);
-      bool covered = at >= 0 && at + n_seq <= tile_valid(*ps, k, q);
+      bool covered = at >= 0 && at + b.seq <= tile_valid(*ps, k, q);
       int64_t first = at * ps->stride[q];
       if (ps->rank == 2) {
-        const int64_t b = tile_start(s, k, 0) - tile_start(*ps, k, 0);
-        covered &= b >= 0 && b + tile_valid(s, k, 0) <= tile_valid(*ps, k, 0);
-        first += b * ps->stride[0];
-        j.pos_outer = ps->stride[0];
+        const int64_t row = tile_start(s, k, 0) - tile_start(*ps, k, 0);
+        covered &= row >= 0 && row + tile_valid(s, k, 0) <= tile_valid(*ps, k, 0);
+        first += row * ps->stride[0];
       }
       if (!covered)
         return fail(MMR_INVALID_ARGUMENT, "device %lld holds positions of another part of the sequence than its tile",
                     (long long)(s.dev_start + k));
-      j.positions = reinterpret_cast<const int32_t*>(mmr::store_tile(positions, k)) + first;
-      j.pos_seq = ps->stride[q];
+      b.positions = reinterpret_cast<const int32_t*>(mmr::store_tile(positions, k)) + first;
     }
-    l.jobs.push_back(j);
-    dims.push_back(s.size[s.rank - 1]);
-    turned.push_back(j.src == j.dst ? 2 : 1);
+    in_place &= b.src == b.dst;
+    l.buffers.push_back(b);
   }
-  if (int rc = shape_jobs(&l, dims, turned, s.itemsize)) return rc;
   mmr::context_hash(ctx, 21, {static_cast<uint64_t>(mmr::store_ordinal(x)), static_cast<uint64_t>(mmr::store_ordinal(out)), flags});
-  return launch_jobs(ctx, &l);
+  return launch_rows(ctx, &l, {Row{s.size[s.rank - 1], true, in_place}}, s.itemsize);
+} catch (...) {
+  return exception_status();
 }
 
 int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* begins, int32_t n, int32_t k_pool, mmr_store* k,
-                    int32_t v_pool, mmr_store* v, mmr_rotary* rotary, mmr_store* q, mmr_store* q_out) {
+                    int32_t v_pool, mmr_store* v, mmr_rotary* rotary, mmr_store* q, mmr_store* q_out) try {
   if (!pages) return fail(MMR_INVALID_ARGUMENT, "null page cache");
   mmr_context* ctx = pages->owner;
   mmr::ContextLock lock(ctx);
@@ -550,10 +588,9 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
   if ((q == nullptr) != (q_out == nullptr)) return fail(MMR_INVALID_ARGUMENT, "q and q_out come together");
   if (q && !rotary) return fail(MMR_INVALID_ARGUMENT, "q without a rotary plan");
   if (v && v_pool == k_pool) return fail(MMR_INVALID_ARGUMENT, "k and v go to the same pool");
-  RotaryLaunch l;
+  mmr::RotaryLaunch l;
   set_plan(&l, rotary, false);
-  std::vector<int64_t> dims;
-  std::vector<int> turned;
+  std::vector<Row> rows;
   int64_t tokens = -1;
   int32_t dtype = -1;
   int itemsize = 0;
@@ -573,28 +610,32 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
   };
   auto add = [&](const mmr_store* s, const Side* pool, const std::vector<char*>* pool_tiles, const mmr_store* out, bool turn) {
     const Side& d = mmr::store_side(s);
-    for (int64_t dev = 0; dev < d.dev_count; ++dev) {
-      mmr::RotaryJob j{};
-      j.src = mmr::store_tile(s, dev);
-      j.tokens = static_cast<uint32_t>(d.size[0]);
-      j.seq = j.tokens;
-      j.heads = static_cast<uint32_t>(tile_valid(d, dev, 1));
-      if (j.tokens == 0 || j.heads == 0) continue;
-      j.src_seq = d.stride[0] * d.itemsize, j.src_head = d.stride[1] * d.itemsize;
-      if (pool) {
-        j.paged = 1;
-        j.dst = (*pool_tiles)[static_cast<size_t>(dev)];
-        j.dst_outer = pool->shard_bytes / pool->size[0];
-        j.dst_seq = pool->stride[1] * pool->itemsize, j.dst_head = pool->stride[2] * pool->itemsize;
-      } else {
-        j.paged = 2;
-        j.dst = mmr::store_tile(out, dev);
-        j.dst_seq = j.src_seq, j.dst_head = j.src_head;
-      }
-      l.jobs.push_back(j);
-      dims.push_back(d.size[2]);
-      turned.push_back(!turn ? 0 : j.src == j.dst ? 2 : 1);
+    if (d.size[0] == 0 || d.size[1] == 0) return;
+    mmr::RotaryShape j{};
+    j.tokens = j.seq = static_cast<uint32_t>(d.size[0]);
+    j.heads = static_cast<uint32_t>(d.ext[1]);
+    j.src_seq = d.stride[0] * d.itemsize, j.src_head = d.stride[1] * d.itemsize;
+    if (pool) {
+      j.paged = 1;
+      j.dst_outer = pool->shard_bytes / pool->size[0];
+      j.dst_seq = pool->stride[1] * pool->itemsize, j.dst_head = pool->stride[2] * pool->itemsize;
+    } else {
+      j.paged = 2;
+      j.dst_seq = j.src_seq, j.dst_head = j.src_head;
     }
+    bool in_place = !pool;
+    for (int64_t dev = 0; dev < d.dev_count; ++dev) {
+      mmr::RotaryBuffer b{};
+      b.src = mmr::store_tile(s, dev);
+      b.dst = pool ? (*pool_tiles)[static_cast<size_t>(dev)] : mmr::store_tile(out, dev);
+      b.outer = 1, b.seq = j.seq, b.heads = static_cast<uint32_t>(tile_valid(d, dev, 1));
+      b.shape = static_cast<uint32_t>(l.shapes.size());
+      if (b.heads == 0) continue;
+      in_place &= b.src == b.dst;
+      l.buffers.push_back(b);
+    }
+    l.shapes.push_back(j);
+    rows.push_back(Row{d.size[2], turn, in_place});
     vectors &= vector_rows(turn ? rotary->dim : 0, l.interleaved, d.size[2], d.itemsize);
   };
   auto add_pool = [&](const mmr_store* s, int32_t pool, bool turn, const char* what) {
@@ -628,15 +669,16 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
   if (int rc = add_pool(k, k_pool, rotary != nullptr, "k")) return rc;
   if (v)
     if (int rc = add_pool(v, v_pool, false, "v")) return rc;
-  if (n == 0 || l.jobs.empty()) return MMR_OK;
+  if (n == 0 || l.buffers.empty()) return MMR_OK;
   l.type = rotary ? dtype : -1;
   l.vectors = vectors;
   const mmr::PageState& st = pages->state;
-  l.args.pages = {st.table, st.lengths, sequences, begins, pages->work.header + mmr::kPageStatus, n, st.S, st.B, st.P, st.T,
+  l.pages = {st.table, st.lengths, sequences, begins, pages->work.header + mmr::kPageStatus, n, st.S, st.B, st.P, st.T,
                   st.capacity, st.div_T};
-  if (int rc = shape_jobs(&l, dims, turned, itemsize)) return rc;
   mmr::context_hash(ctx, 22, {static_cast<uint64_t>(mmr::store_ordinal(k)), static_cast<uint64_t>(k_pool), static_cast<uint64_t>(n)});
-  return launch_jobs(ctx, &l);
+  return launch_rows(ctx, &l, rows, itemsize);
+} catch (...) {
+  return exception_status();
 }
 
 }  // extern "C"

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <vector>
+
 #include "page_ops.h"
 #include "rotary_ops.h"
 
@@ -30,9 +32,17 @@ hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_
                             const PageMoveLaunch& mv, hipStream_t stream);
 hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream);
 
-// `type`: MMR_F32, MMR_BF16 or MMR_F16; -1: rows only move (no job turns anything).  past_caches: how results are stored.
-hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, bool past_caches,
-                         hipStream_t stream);
+// One call's rows: at most kRotaryShapes shapes, any number of buffers (several launches if there are many).
+struct RotaryLaunch {
+  RotaryAngles angles{};
+  RotaryPages pages{};
+  std::vector<RotaryShape> shapes;
+  std::vector<RotaryBuffer> buffers;
+  int type = -1;  // MMR_F32, MMR_BF16 or MMR_F16; -1: rows only move (nothing is turned)
+  bool vectors = false, interleaved = false;
+  bool past_caches = false;  // how results are stored
+};
+hipError_t launch_rotary(const RotaryLaunch& l, int* launches, hipStream_t stream);
 
 }  // namespace mmr
 

@@ -189,12 +189,58 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState 
 // STREAM: a launch that writes more than the caches keep for a reader writes past them (queries, keys and values of 18,001
 // tokens, 443 MB in all: 82.4 -> 79.3 us; the gradient of bf16 [4,32,2048,128] 23.9 -> 20.7 us); what a small one
 // writes, a decode step's queries and keys, stays for the kernel that reads it next.
-template <class T, int VEC, bool INTERLEAVED, bool STREAM>
-__global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(RotaryArgs a) {
+template <class T, int VEC, bool INTERLEAVED, bool STREAM, class Args>
+__global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(Args a) {
   Workgroup<kRotaryThreads> x(nullptr);
-  const RotaryJob& j = a.jobs[blockIdx.y];
+  const RotaryBuffer& b = a.buffers[blockIdx.y];
+  const RotaryShape& j = a.shapes[Args::kShapes == 1 ? 0 : b.shape];
   if (x.block >= j.blocks) return;  // uniform over the workgroup
-  rotary_block<DeviceMem<false, STREAM>, T, VEC, INTERLEAVED>(x, a, j);
+  rotary_block<DeviceMem<false, STREAM>, T, VEC, INTERLEAVED>(x, a.angles, a.pages, j, b);
+}
+
+template <class Args>
+hipError_t launch_rotary_args(const RotaryLaunch& l, const Args& args, uint32_t blocks, int n, hipStream_t stream) {
+  const dim3 grid(blocks, static_cast<uint32_t>(n)), threads(kRotaryThreads);
+#define MMR_ROTARY(T, V, I)                                                                                           \
+  do {                                                                                                               \
+    if (l.past_caches) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, true, Args>), grid, threads, 0, stream, args);    \
+    else hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, false, Args>), grid, threads, 0, stream, args);                 \
+  } while (0)
+#define MMR_ROTARY_TYPE(T, V)                                       \
+  do {                                                              \
+    if (l.vectors && l.interleaved) MMR_ROTARY(T, V, true);         \
+    else if (l.vectors) MMR_ROTARY(T, V, false);                    \
+    else if (l.interleaved) MMR_ROTARY(T, 1, true);                 \
+    else MMR_ROTARY(T, 1, false);                                   \
+  } while (0)
+  switch (l.type) {
+    case MMR_F32: MMR_ROTARY_TYPE(RotaryF32, 4); break;
+    case MMR_BF16: MMR_ROTARY_TYPE(RotaryBF16, 8); break;
+    case MMR_F16: MMR_ROTARY_TYPE(RotaryF16, 8); break;
+    default:
+      if (l.vectors) MMR_ROTARY(RotaryRaw, 16, false);
+      else MMR_ROTARY(RotaryRaw, 1, false);
+  }
+#undef MMR_ROTARY_TYPE
+#undef MMR_ROTARY
+  return hipGetLastError();
+}
+
+// Buffers [at, at + n) of a launch, with the shapes they have.
+template <class Args>
+hipError_t launch_rotary_part(const RotaryLaunch& l, size_t at, int n, hipStream_t stream) {
+  Args args;
+  args.angles = l.angles;
+  args.pages = l.pages;
+  for (int i = 0; i < Args::kShapes; ++i) args.shapes[i] = i < static_cast<int>(l.shapes.size()) ? l.shapes[static_cast<size_t>(i)] : RotaryShape{};
+  uint32_t blocks = 0;
+  for (int i = 0; i < Args::kBuffers; ++i) {
+    args.buffers[i] = i < n ? l.buffers[at + static_cast<size_t>(i)] : RotaryBuffer{};
+    if (i >= n) continue;
+    const uint32_t mine = l.shapes[args.buffers[i].shape].blocks;
+    blocks = mine > blocks ? mine : blocks;
+  }
+  return launch_rotary_args(l, args, blocks, n, stream);
 }
 
 // The launch before a plan, where the pool is more than a plan scans itself.
@@ -207,10 +253,12 @@ hipError_t launch_scan(const PageState& st, const PageWork& w, bool live, hipStr
 // Workgroups of a move: one per chunk up to this many, which then loop.
 constexpr uint64_t kMaxMoveBlocks = 1u << 18;
 
-// Up to so many pages the plan of a compact lists the moves itself, in at most 8 rounds.
+// Up to so many pages the plan of a compact lists the moves itself, in at most 8 rounds (compact of 16,384 pages of 256
+// bytes: 19.9 us, with a launch for the list 21.8; of 32,768: 30.1 and 23.7).
 constexpr int32_t kCompactWhole = 16384;
-// Up to so many chunks a copy of few pairs is one launch, whose workgroups each check all pairs.
-constexpr uint64_t kFewChunks = 4096;
+// Up to so many chunks a copy of few pairs is one launch, whose workgroups each check all pairs (64 chunks: 4.6 us, in
+// two launches 6.9; 1,024 chunks of 64 pairs: 9.5 and 8.1; 4,096: 23.3 and 17.2).
+constexpr uint64_t kFewChunks = 256;
 
 template <int KIND>
 hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
@@ -282,6 +330,8 @@ hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_
     else hipLaunchKernelGGL(mmr_page_copy_few_kernel<false>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
     return hipGetLastError();
   }
+  // in the order of the destinations 512 pages of 32 KiB in each of 48 buffers take 293 us, in the caller's 308; where the pairs
+  // are few among the pages the pass over these costs more than it gives (512 of 20,000: 59 us, sorted 69)
   const bool sorted = st.P / 8 <= n;
   hipLaunchKernelGGL(mmr_page_copy_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, src, dst, n, sorted);
   if (hipError_t e = hipGetLastError()) return e;
@@ -294,35 +344,20 @@ hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t
   return hipGetLastError();
 }
 
-hipError_t launch_rotary(const RotaryArgs& args, int n_jobs, int type, bool vectors, bool interleaved, bool past_caches,
-                         hipStream_t stream) {
-  uint32_t blocks = 0;
-  for (int i = 0; i < n_jobs; ++i) blocks = args.jobs[i].blocks > blocks ? args.jobs[i].blocks : blocks;
-  if (!blocks) return hipSuccess;
-  const dim3 grid(blocks, static_cast<uint32_t>(n_jobs)), threads(kRotaryThreads);
-#define MMR_ROTARY(T, V, I)                                                                                     \
-  do {                                                                                                         \
-    if (past_caches) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, true>), grid, threads, 0, stream, args);   \
-    else hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, false>), grid, threads, 0, stream, args);              \
-  } while (0)
-#define MMR_ROTARY_TYPE(T, V)                                     \
-  do {                                                            \
-    if (vectors && interleaved) MMR_ROTARY(T, V, true);           \
-    else if (vectors) MMR_ROTARY(T, V, false);                    \
-    else if (interleaved) MMR_ROTARY(T, 1, true);                 \
-    else MMR_ROTARY(T, 1, false);                                 \
-  } while (0)
-  switch (type) {
-    case MMR_F32: MMR_ROTARY_TYPE(RotaryF32, 4); break;
-    case MMR_BF16: MMR_ROTARY_TYPE(RotaryBF16, 8); break;
-    case MMR_F16: MMR_ROTARY_TYPE(RotaryF16, 8); break;
-    default:
-      if (vectors) MMR_ROTARY(RotaryRaw, 16, false);
-      else MMR_ROTARY(RotaryRaw, 1, false);
+hipError_t launch_rotary(const RotaryLaunch& l, int* launches, hipStream_t stream) {
+  *launches = 0;
+  for (size_t at = 0; at < l.buffers.size();) {
+    const size_t left = l.buffers.size() - at;
+    const int n = static_cast<int>(left < RotaryManyBuffers::kBuffers ? left : RotaryManyBuffers::kBuffers);
+    hipError_t e;
+    if (l.shapes.size() == 1 && n <= RotaryOneShape::kBuffers) e = launch_rotary_part<RotaryOneShape>(l, at, n, stream);
+    else if (n <= RotaryFewBuffers::kBuffers) e = launch_rotary_part<RotaryFewBuffers>(l, at, n, stream);
+    else e = launch_rotary_part<RotaryManyBuffers>(l, at, n, stream);
+    if (e) return e;
+    *launches += 1;
+    at += static_cast<size_t>(n);
   }
-#undef MMR_ROTARY_TYPE
-#undef MMR_ROTARY
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 }  // namespace mmr

@@ -103,7 +103,8 @@ MMR_HD void page_scan_segment(X& x, const PageState& st, const PageWork& w, int3
   if (x.tid == 0) w.seg_free[segment] = total;
 }
 
-// Up to so many segments a plan scans itself.
+// Up to so many segments a plan scans itself (compact of 8,192 pages, two segments: 16.2 us, with a launch for the scan
+// 17.9; of 16,384, four: 21.9 and 19.9).
 constexpr int32_t kPlanScans = 2;
 
 template <class X>

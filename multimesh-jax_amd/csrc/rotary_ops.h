@@ -23,28 +23,40 @@
 namespace mmr {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryHeads = 4;   // heads a lane takes with one set of angles
-constexpr int kRotaryMaxJobs = 16;
+constexpr int kRotaryHeads = 4;    // heads a lane takes with one set of angles
+constexpr int kRotaryShapes = 3;   // shapes of one call (queries, keys, values)
 
-// One buffer: rows of `dim` elements over outer x seq tokens and heads.  Strides in bytes.
-struct RotaryJob {
-  const char* src;
-  char* dst;
+// n / d for n < 256 and 1 <= d <= 256: exact, as n * (mul * d - 2^16) < n * d < 2^16.
+MMR_HD uint32_t small_div(uint32_t n, uint32_t mul) { return (n * mul) >> 16; }
+inline uint32_t make_small_div(uint32_t d) { return (65536u + d - 1) / d; }
+
+// Rows of `dim` elements over outer x seq tokens and heads, and how they are dealt to workgroups: the extents of a tile,
+// the same on every device.  Strides in bytes.
+struct RotaryShape {
   int64_t src_outer, src_seq, src_head;
   int64_t dst_outer, dst_seq, dst_head;  // paged: dst_outer is the page, dst_seq the token of a page
-  const int32_t* positions;              // null: base + index along seq
-  int64_t pos_outer, pos_seq;
+  int64_t pos_outer, pos_seq;            // in elements
+  uint32_t tokens, seq, heads;           // tokens = outer * seq
+  uint32_t rot_units, units;             // units of a row: rotated ones first
+  uint32_t head_groups;                  // workgroups along the heads
+  uint32_t blocks;                       // workgroups of a buffer
+  uint32_t mul_lanes, mul_head_lanes;    // small_div by the two
+  uint16_t lanes;                        // lanes of a row: min(units, kRotaryThreads)
+  uint16_t head_lanes;                   // rows of a workgroup along the heads ...
+  uint16_t token_lanes;                  // ... and along the tokens
+  uint16_t head_steps;                   // heads a lane takes, head_lanes apart
+  uint32_t paged;                        // 1: into pages; 2: by the positions of a paged write, beside the source
+  FastDiv div_seq, div_head_groups;
+};
+
+// One buffer of that shape, and how much of the tile is not padding.
+struct RotaryBuffer {
+  const char* src;
+  char* dst;
+  const int32_t* positions;  // null: base + index along seq
   int64_t base;
-  uint32_t tokens, seq, heads;  // tokens = outer * seq
-  uint32_t rot_units, units;    // units of a row: rotated ones first
-  uint32_t lanes;               // lanes of a row: min(units, kRotaryThreads)
-  uint32_t head_lanes;          // rows of a workgroup along the heads ...
-  uint32_t token_lanes;         // ... and along the tokens
-  uint32_t head_steps;          // heads a lane takes, head_lanes apart
-  uint32_t head_groups;         // workgroups along the heads
-  uint32_t blocks;              // workgroups of this job
-  uint32_t paged;
-  FastDiv div_seq, div_lanes, div_head_lanes, div_head_groups;
+  uint32_t outer, seq, heads;
+  uint32_t shape;
 };
 
 // Where new tokens of a paged write go.
@@ -59,14 +71,28 @@ struct RotaryPages {
   FastDiv div_T;
 };
 
-struct RotaryArgs {
+struct RotaryAngles {
   const uint64_t* frequency;  // turns per position, 0.64 fixed point
   float magnitude;
   float sine;                 // magnitude, negative for the gradient
   uint32_t half;              // R / 2
-  RotaryPages pages;
-  RotaryJob jobs[kRotaryMaxJobs];
 };
+
+// The argument block of a launch of up to N buffers of up to S shapes.  Its size is much of what a launch of few rows
+// costs: with 3 KB (16 buffers, each with all a shape holds) a layer of a decode step took 6.0 us, and 28 us waited for
+// alone; with 0.7 KB 5.7 and 19.  So there are three: one shape on up to 8 devices (0.6 KB), queries, keys and values on
+// one device (0.7 KB), and everything else (1.6 KB).
+template <int S, int N>
+struct RotaryArgs {
+  static constexpr int kShapes = S, kBuffers = N;
+  RotaryAngles angles;
+  RotaryPages pages;
+  RotaryShape shapes[S];
+  RotaryBuffer buffers[N];
+};
+typedef RotaryArgs<1, 8> RotaryOneShape;
+typedef RotaryArgs<kRotaryShapes, 4> RotaryFewBuffers;
+typedef RotaryArgs<kRotaryShapes, 24> RotaryManyBuffers;
 
 // sin and cos of `turns` / 2^32 of a turn
 MMR_HD void turn_sincos(uint32_t turns, float* s, float* c) {
@@ -184,21 +210,22 @@ MMR_HD bool rotary_place(X& x, const RotaryPages& pg, int32_t wave_token, int32_
   return *bad == 0;
 }
 
-// Lane (row, unit) of workgroup `block` of a job.  A unit is what a lane turns: the two vectors that hold VEC pairs, or,
+// Lane (row, unit) of workgroup `block` of a buffer.  A unit is what a lane turns: the two vectors that hold VEC pairs, or,
 // interleaved, one vector of VEC / 2 pairs; in the rest of the row it is one vector.  The rows are loaded before the
 // position is looked up: the look-up is a chain of four loads.
 template <class M, class T, int VEC, bool INTERLEAVED, class X>
-MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
+MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, const RotaryShape& j, const RotaryBuffer& b) {
   constexpr int kVecBytes = VEC * T::kBytes;
   constexpr bool kTwo = T::kBytes > 1 && (!INTERLEAVED || VEC == 1);  // a unit of the rotated part is two vectors
   constexpr int kPairs = INTERLEAVED && VEC > 1 ? VEC / 2 : VEC;      // and so many pairs
   const uint32_t group = fdiv(x.block, j.div_head_groups), hg = x.block - group * j.head_groups;
-  const uint32_t row = fdiv(static_cast<uint32_t>(x.tid), j.div_lanes), lane = static_cast<uint32_t>(x.tid) - row * j.lanes;
-  const uint32_t tsub = fdiv(row, j.div_head_lanes), hsub = row - tsub * j.head_lanes;
+  const uint32_t row = small_div(static_cast<uint32_t>(x.tid), j.mul_lanes), lane = static_cast<uint32_t>(x.tid) - row * j.lanes;
+  const uint32_t tsub = small_div(row, j.mul_head_lanes), hsub = row - tsub * j.head_lanes;
   const uint32_t token = group * j.token_lanes + tsub;
-  const bool on = tsub < j.token_lanes && token < j.tokens;
-  const uint32_t outer = fdiv(on ? token : 0u, j.div_seq), seq = (on ? token : 0u) - outer * j.seq;
-  const char* const src = j.src + (static_cast<int64_t>(outer) * j.src_outer + static_cast<int64_t>(seq) * j.src_seq);
+  const bool inside = tsub < j.token_lanes && token < j.tokens;
+  const uint32_t outer = fdiv(inside ? token : 0u, j.div_seq), seq = (inside ? token : 0u) - outer * j.seq;
+  const bool on = inside && outer < b.outer && seq < b.seq;
+  const char* const src = b.src + (static_cast<int64_t>(outer) * j.src_outer + static_cast<int64_t>(seq) * j.src_seq);
   const uint32_t h0 = hg * j.head_lanes * j.head_steps + hsub;
 
   // byte offsets in a row of the two vectors of a unit (of the one, for units of the rest)
@@ -215,7 +242,7 @@ MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
 #pragma unroll
     for (uint32_t k = 0; k < kRotaryHeads; ++k) {
       const uint32_t h = h0 + k * j.head_lanes;
-      if (k < j.head_steps && h < j.heads) {
+      if (k < j.head_steps && h < b.heads) {
         va[k].template load<M>(M::cplace(src + (h * j.src_head + off_a)));
         if (kTwo && unit < j.rot_units) vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
       }
@@ -234,26 +261,26 @@ MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
   }
 
   int64_t position = 0;
-  char* dst = j.dst;
+  char* dst = b.dst;
   if (j.paged) {
     // the token of the wave's first lane, for all lanes to look up together
-    const uint32_t first = fdiv(fdiv(static_cast<uint32_t>(x.tid) & ~63u, j.div_lanes), j.div_head_lanes);
+    const uint32_t first = small_div(small_div(static_cast<uint32_t>(x.tid) & ~63u, j.mul_lanes), j.mul_head_lanes);
     const int32_t wave_token = static_cast<int32_t>(group * j.token_lanes + first);
     int32_t page = 0, in_page = 0;
     uint32_t bad = 0;
     // lanes without a token ask for their wave's first one and go no further
-    const bool there = rotary_place(x, a.pages, wave_token, on ? static_cast<int32_t>(token) : wave_token, &position, &page, &in_page, &bad);
+    const bool there = rotary_place(x, pages, wave_token, on ? static_cast<int32_t>(token) : wave_token, &position, &page, &in_page, &bad);
     if (!on) return;
     if (!there) {
-      if (bad && lane == 0 && hsub == 0) x.atomic_or(a.pages.status, static_cast<int32_t>(bad));
+      if (bad && lane == 0 && hsub == 0) x.atomic_or(pages.status, static_cast<int32_t>(bad));
       return;
     }
     if (j.paged == 1) dst += static_cast<int64_t>(page) * j.dst_outer + static_cast<int64_t>(in_page) * j.dst_seq;
     else dst += static_cast<int64_t>(seq) * j.dst_seq;  // queries: turned by the token's position, written beside it
   } else {
     if (!on) return;
-    position = j.positions ? j.positions[static_cast<int64_t>(outer) * j.pos_outer + static_cast<int64_t>(seq) * j.pos_seq]
-                           : j.base + seq;
+    position = b.positions ? b.positions[static_cast<int64_t>(outer) * j.pos_outer + static_cast<int64_t>(seq) * j.pos_seq]
+                           : b.base + seq;
     dst += static_cast<int64_t>(outer) * j.dst_outer + static_cast<int64_t>(seq) * j.dst_seq;
   }
 
@@ -290,7 +317,7 @@ MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
           }
         }
         const uint32_t h = h0 + k * j.head_lanes;
-        if (h < j.heads) {
+        if (h < b.heads) {
           va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
           if (kTwo) vb[k].template store<M>(M::place(dst + (h * j.dst_head + off_b)));
         }
@@ -299,7 +326,7 @@ MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
 #pragma unroll
       for (uint32_t k = 0; k < kRotaryHeads; ++k) {
         const uint32_t h = h0 + k * j.head_lanes;
-        if (k < j.head_steps && h < j.heads) va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
+        if (k < j.head_steps && h < b.heads) va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
       }
     }
     unit += j.lanes;
@@ -309,29 +336,30 @@ MMR_HD void rotary_block(X& x, const RotaryArgs& a, const RotaryJob& j) {
   }
 }
 
-// How a job's rows are dealt to workgroups; returns how many that takes.  `spread`: one head a lane, for launches that
-// would not fill the chip.
-inline uint64_t rotary_shape(RotaryJob* j, uint32_t rot_units, uint32_t rest_units, bool heads_adjacent, bool spread) {
+// How the rows of a shape are dealt to workgroups; returns how many that takes.  `spread`: one head a lane, for launches
+// that would not fill the chip.
+inline uint64_t rotary_shape(RotaryShape* j, uint32_t rot_units, uint32_t rest_units, bool heads_adjacent, bool spread) {
   const uint32_t threads = kRotaryThreads;
   j->rot_units = rot_units;
   j->units = rot_units + rest_units;
-  j->lanes = j->units < threads ? j->units : threads;
-  const uint32_t rows = threads / j->lanes;
+  const uint32_t lanes = j->units < threads ? j->units : threads;
+  const uint32_t rows = threads / lanes;
   const uint32_t want = spread ? 1u : static_cast<uint32_t>(kRotaryHeads);
-  j->head_lanes = heads_adjacent || spread ? (j->heads + want - 1) / want : 1;
-  if (j->head_lanes > rows) j->head_lanes = rows;
-  j->token_lanes = rows / j->head_lanes;
-  if (spread && j->token_lanes > 1 && j->tokens < 1024) j->token_lanes = 1;
-  const uint32_t steps = (j->heads + j->head_lanes - 1) / j->head_lanes;
+  uint32_t head_lanes = heads_adjacent || spread ? (j->heads + want - 1) / want : 1;
+  if (head_lanes > rows) head_lanes = rows;
+  uint32_t token_lanes = rows / head_lanes;
+  if (spread && j->tokens < 1024) token_lanes = 1;
+  const uint32_t steps = (j->heads + head_lanes - 1) / head_lanes;
   const uint32_t groups = (steps + want - 1) / want;
-  j->head_steps = (steps + groups - 1) / groups;  // 5 heads go as 3 and 2, not as 4 and 1
-  const uint32_t per = j->head_lanes * j->head_steps;
+  const uint32_t head_steps = (steps + groups - 1) / groups;  // 5 heads go as 3 and 2, not as 4 and 1
+  const uint32_t per = head_lanes * head_steps;
   j->head_groups = (j->heads + per - 1) / per;
-  const uint64_t blocks = (static_cast<uint64_t>(j->tokens) + j->token_lanes - 1) / j->token_lanes * j->head_groups;
+  const uint64_t blocks = (static_cast<uint64_t>(j->tokens) + token_lanes - 1) / token_lanes * j->head_groups;
   j->blocks = static_cast<uint32_t>(blocks);
+  j->lanes = static_cast<uint16_t>(lanes), j->head_lanes = static_cast<uint16_t>(head_lanes);
+  j->token_lanes = static_cast<uint16_t>(token_lanes), j->head_steps = static_cast<uint16_t>(head_steps);
+  j->mul_lanes = make_small_div(lanes), j->mul_head_lanes = make_small_div(head_lanes);
   j->div_seq = make_fastdiv(j->seq);
-  j->div_lanes = make_fastdiv(j->lanes);
-  j->div_head_lanes = make_fastdiv(j->head_lanes);
   j->div_head_groups = make_fastdiv(j->head_groups);
   return blocks;
 }

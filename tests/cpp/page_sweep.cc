@@ -58,12 +58,12 @@ struct Lanes {
     return before;
   }
   uint32_t any(uint32_t f) {
-    int32_t total = 0;
-    uint32_t all = 0;
-    for (int b = 0; b < 10; ++b) {
-      scan<int32_t>((f >> b) & 1, &total);
-      all |= total ? 1u << b : 0;
-    }
+    if (tid == 0) s->flags = 0;
+    sync();
+    __atomic_fetch_or(&s->flags, f, __ATOMIC_SEQ_CST);
+    sync();
+    const uint32_t all = __atomic_load_n(&s->flags, __ATOMIC_SEQ_CST);
+    sync();
     return all;
   }
   bool all(bool v) { return v; }  // a lane is a wave of its own here
@@ -478,16 +478,16 @@ void cache_case(uint64_t seed) {
       if (count && count <= kFewPairs && pick(0, 1)) {
         int32_t pairs[2 * kFewPairs];
         const uint32_t items = static_cast<uint32_t>(count) * c.mover.n_buffers * c.mover.chunks;
-        std::vector<char> ok(items);
-        launch<kFewPairs>(items, [&](Lanes<kFewPairs>& x) {
+        std::vector<char> ok(std::min(items, 5u));  // the first workgroups check, one after the other
+        launch<kFewPairs>(static_cast<uint32_t>(ok.size()), [&](Lanes<kFewPairs>& x) {
           const bool go = page_copy_few(x, c.st, c.w, pairs, sa.p, sb.p, count);
           if (x.tid == 0) ok[x.block] = go;
-          // by one thread: vectors that slide back repeat their neighbours' bytes, which the thread sanitizer takes for a race
-          for (uint32_t t = 0; go && x.tid == 0 && t < static_cast<uint32_t>(kPageThreads); ++t)
-            c.chunk(x.block, static_cast<uint32_t>(count), t, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; });
         });
         for (char g : ok)
           if (g != ok[0]) die("workgroups disagree");
+        for (uint32_t item = 0; ok[0] && item < items; ++item)
+          for (uint32_t t = 0; t < static_cast<uint32_t>(kPageThreads); ++t)
+            c.chunk(item, static_cast<uint32_t>(count), t, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; });
       } else if (count) {
         const bool sorted = pick(0, 1);
         launch<K>(1, [&](Lanes<K>& x) { page_copy_plan(x, c.st, c.w, sa.p, sb.p, count, sorted); });
@@ -552,12 +552,14 @@ void rotary_case(uint64_t seed, double eps) {
   Exact<uint64_t> freq(half);
   for (int i = 0; i < half; ++i) freq[i] = static_cast<uint64_t>(std::ldexp(std::pow(100.0, -static_cast<double>(i) / half) / 6.283185307179586, 62)) * 4;
   const int64_t row = static_cast<int64_t>(dim) * T::kBytes;
-  RotaryArgs a{};
+  RotaryAngles a{};
+  RotaryPages pages{};
+  RotaryShape j{};
+  RotaryBuffer buf{};
   a.frequency = freq.p;
   a.magnitude = 1.25f;
   a.sine = pick(0, 1) ? 1.25f : -1.25f;
   a.half = half;
-  RotaryJob& j = a.jobs[0];
   Exact<char> x(static_cast<size_t>(tokens) * heads * row);
   std::normal_distribution<float> normal;
   for (int64_t i = 0; i < static_cast<int64_t>(tokens) * heads * dim; ++i) {
@@ -573,7 +575,7 @@ void rotary_case(uint64_t seed, double eps) {
   Exact<int32_t> table(S * B), lengths(S), slots(n), begins(n + 1), status(1), positions(tokens);
   Exact<char> pool(paged == 1 ? static_cast<size_t>(P) * Tk * heads * row : 0), out(paged == 1 || in_place ? 0 : x.n, 0x11);
   std::vector<int32_t> where(tokens, -1), page_of(tokens, -1), row_of(tokens, 0);
-  j.src = x.p;
+  buf.src = x.p;
   uint32_t want_status = 0;
   if (paged) {
     std::vector<int32_t> ids(P);
@@ -612,35 +614,41 @@ void rotary_case(uint64_t seed, double eps) {
         where[t] = p, page_of[t] = page, row_of[t] = p % Tk;
       }
     }
-    a.pages = {table.p, lengths.p, slots.p, begins.p, status.p, n, S, B, P, Tk, B * Tk, make_fastdiv(static_cast<uint32_t>(Tk))};
-    j.dst = paged == 1 ? pool.p : in_place ? x.p : out.p;
+    pages = {table.p, lengths.p, slots.p, begins.p, status.p, n, S, B, P, Tk, B * Tk, make_fastdiv(static_cast<uint32_t>(Tk))};
+    buf.dst = paged == 1 ? pool.p : in_place ? x.p : out.p;
     if (paged == 1) j.dst_outer = Tk * heads * row, j.dst_seq = heads * row, j.dst_head = row;
     else j.dst_seq = j.src_seq, j.dst_head = j.src_head;
   } else {
-    j.dst = in_place ? x.p : out.p;
+    buf.dst = in_place ? x.p : out.p;
     j.dst_outer = j.src_outer, j.dst_seq = j.src_seq, j.dst_head = j.src_head;
     const bool given = pick(0, 1);
-    j.base = pick(-100, 1000000);
+    buf.base = pick(-100, 1000000);
     j.pos_outer = seq, j.pos_seq = 1;
-    if (given) j.positions = positions.p;
+    if (given) buf.positions = positions.p;
     for (int t = 0; t < tokens; ++t) {
       positions[t] = pick(-5, 70000);
-      where[t] = given ? positions[t] : static_cast<int32_t>(j.base + t % seq);
+      where[t] = given ? positions[t] : static_cast<int32_t>(buf.base + t % seq);
     }
   }
   const auto before = x.copy();
-  const bool same = j.dst == x.p;
+  const bool same = buf.dst == x.p;
   const int rot = turn ? (INTERLEAVED && VEC > 1 ? 2 * half : half) / VEC : 0, rest = turn ? (same ? 0 : (dim - 2 * half) / VEC) : dim / VEC;
   rotary_shape(&j, rot, rest, j.src_head <= j.src_seq, spread);
-  const RotaryArgs args = a;
-  launch<kRotaryThreads>(j.blocks, [&](Lanes<kRotaryThreads>& l) { rotary_block<Mem, T, VEC, INTERLEAVED>(l, args, args.jobs[0]); });
+  // in some cases a part of the tile is padding, which stays as it is
+  buf.outer = paged ? 1 : pick(1, outer), buf.seq = paged || pick(0, 1) ? seq : pick(1, seq), buf.heads = pick(0, 1) ? heads : pick(1, heads);
+  for (uint32_t b = 0; b < j.blocks; ++b)  // its lanes wait for nothing, so that one thread can be all of them in turn
+    for (int32_t t = 0; t < kRotaryThreads; ++t) {
+      Lanes<kRotaryThreads> l{t, b, j.blocks, nullptr};
+      rotary_block<Mem, T, VEC, INTERLEAVED>(l, a, pages, j, buf);
+    }
   if (static_cast<uint32_t>(status[0]) != want_status) die("rotary: status", want_status, status[0]);
   std::set<std::pair<int32_t, int32_t>> written;
   for (int t = 0; t < tokens; ++t)
     for (int h = 0; h < heads; ++h) {
       const int64_t at = (t / seq) * j.src_outer + (t % seq) * j.src_seq + h * j.src_head;
       const char* to;
-      const bool skip = paged && page_of[t] < 0;
+      const bool pad = static_cast<uint32_t>(h) >= buf.heads || static_cast<uint32_t>(t % seq) >= buf.seq || static_cast<uint32_t>(t / seq) >= buf.outer;
+      const bool skip = (paged && page_of[t] < 0) || pad;
       if (paged == 1) {
         if (skip) continue;
         to = pool.p + page_of[t] * j.dst_outer + row_of[t] * j.dst_seq + h * j.dst_head;

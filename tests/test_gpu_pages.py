@@ -308,6 +308,10 @@ ROTARY = [
     ((6, 3, 600), 0, 0, 2, None, 600, False, "F32", {}, 1.0, 0),
     ((6, 3, 1100), 0, 0, 1, None, 1100, False, "F32", dict(frequencies=True), 1.0, 9),
     ((7, 2, 2), 0, 0, 1, None, 2, False, "BF16", {}, 1.0, 0),
+    ((40, 3, 16), 0, 0, 20, None, 16, False, "BF16", {}, 1.0, 0),   # 20 buffers: more than one launch takes
+    ((1, 1, 8), 0, 0, 1, None, 8, True, "F16", {}, 1.0, 12345),
+    ((300, 9, 32, 128), 1, 1, 3, None, 128, False, "BF16", {}, 1.0, 7),  # 22 MB
+    ((2, 2100, 33, 128), 1, 2, 1, None, 128, False, "F32", {}, 1.0, 7),  # 71 MB: results past the caches, 33 heads
 ]
 
 
@@ -414,6 +418,9 @@ WRITE = [
     (2, 4, 128, None, False, "BF16", 2, None, 16, [33, 1]),
     (3, 3, 7, None, False, "F8E4M3FN", 1, None, 3, [4, 5, 0]),
     (1, 16, 128, 128, False, "F16", 1, None, 64, [700]),
+    (16, 24, 64, 64, False, "BF16", 8, None, 16, [1, 1, 1, 1, 1]),  # 24 buffers: more than one launch takes
+    (2, 2, 32, 32, False, "F32", 1, None, 2, [1] * 130),            # more sequences than a wave has lanes
+    (3, 3, 32, 16, True, "F32", 1, None, 2, [0, 2] * 70 + [0, 0, 5]),
 ]
 
 
@@ -768,6 +775,7 @@ def test_calls_that_the_host_refuses():
         assert c.stats["kernel_launches"] == launches
         for call, error in ((lambda: s["cache"].Free([0]), TypeError), (lambda: s["cache"].Free(np.zeros(1, np.int32)), TypeError),
                             (lambda: s["cache"].Free(s["table"]), ValueError), (lambda: s["cache"].Free(s["f32"]), ValueError),
+                            (lambda: s["cache"].Free(whole(other, z(1))), ValueError),
                             (lambda: s["cache"].Extend(s["one"], s["two"]), ValueError),
                             (lambda: s["cache"].Write(s["one"], s["one"], 0, s["k"]), ValueError),
                             (lambda: c.CreateRotary(8, frequencies=[1.0]), ValueError)):

@@ -13,7 +13,7 @@ from multimesh_jax_amd import _binding as B
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("program,rounds", [("page_sweep", 60), ("page_sweep_threads", 25)])
+@pytest.mark.parametrize("program,rounds", [("page_sweep", 60), ("page_sweep_threads", 20)])
 def test_kernels_under_the_sanitizers(program, rounds):
     p = subprocess.run([os.path.join(HERE, "cpp", program), str(rounds)], capture_output=True, text=True, timeout=600)
     assert p.returncode == 0 and p.stdout.strip().endswith("OK"), p.stdout + p.stderr
