@@ -530,7 +530,7 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  * nothing, copies nothing from the host and may be captured into a HIP graph; calls of one cache are ordered by the
  * context's stream, and graphs captured from one cache must not run at the same time, as they share its tables and
  * workspace.  (The first call after a pool was offloaded and reloaded enters its buffers anew and is refused while
- * capturing, and a graph captured before that must not be replayed.)
+ * capturing, and a graph captured before that, or from a handle that was destroyed since, must not be replayed.)
  *
  * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
  * so on.  extend, fork and copy check all their entries first and change nothing at all if one is bad; the reason is
@@ -612,7 +612,9 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
  * begins[i]).  begins: n + 1 ascending values; tokens before the first and after the last are padding and left out.  k
  * goes to pool k_pool, v (or NULL) to pool v_pool: stores [tokens, heads, dim], heads sharded as in the pool.  With a
  * rotary plan k is turned on its way, and q (any heads, [tokens, heads, dim], or NULL) is turned into q_out (or in
- * place).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type. */
+ * place).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.  Tokens of an entry whose
+ * sequence or page is not there, or that are more than the sequence holds, are left out (q_out too), the others are
+ * written; the reason is kept for mmr_pages_status. */
 int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* begins, int32_t n, int32_t k_pool, mmr_store* k,
                     int32_t v_pool, mmr_store* v, mmr_rotary* rotary, mmr_store* q, mmr_store* q_out);
 

@@ -212,6 +212,7 @@ struct mmr_store {
   size_t bytes = 0;
   std::vector<char*> adopted;  // caller-owned buffers, one per device (mmr_store_adopt)
   char* host = nullptr;        // pinned host copy while the store is offloaded (the device buffers are gone then)
+  bool watched = false;        // another operator's handle keeps this store's addresses
   mmr_context* owner = nullptr;
 
   // Replicated stores keep the tiles of one replica together (replica after replica) whatever the order of the device
@@ -265,7 +266,7 @@ struct mmr_context {
   std::unordered_map<size_t, std::vector<char*>> free_pool;
   size_t free_pool_bytes = 0;
   std::unordered_map<int64_t, std::unique_ptr<mmr_store>> stores;
-  uint64_t store_epoch = 0;  // bumped when a store is freed, offloaded or reloaded
+  uint64_t store_epoch = 0;  // bumped when a watched store is freed, offloaded or reloaded
   std::unordered_map<mmr::Attachment*, std::unique_ptr<mmr::Attachment>> attachments;  // handles of other operators
   int64_t next_ordinal = 0;
   mmr_context_stats stats{};
@@ -1275,6 +1276,7 @@ void context_attach(mmr_context* ctx, std::unique_ptr<Attachment> a) {
 }
 void context_detach(mmr_context* ctx, Attachment* a) { ctx->attachments.erase(a); }
 uint64_t context_store_epoch(mmr_context* ctx) { return ctx->store_epoch; }
+void context_watch(mmr_store* store) { store->watched = true; }
 mmr_store* context_find_store(mmr_context* ctx, int64_t id) {
   auto it = ctx->stores.find(id);
   return it == ctx->stores.end() ? nullptr : it->second.get();
@@ -1543,7 +1545,7 @@ int mmr_store_free(mmr_context* ctx, mmr_store* store, int32_t keep_in_cache) {
     ctx->stats.bytes_allocated -= static_cast<int64_t>(store->bytes);
   }
   ctx->stats.stores_live -= 1;
-  ctx->store_epoch += 1;
+  ctx->store_epoch += store->watched;
   ctx->stores.erase(store->id);
   return MMR_OK;
 }
@@ -1750,7 +1752,7 @@ int mmr_store_offload(mmr_context* ctx, mmr_store* store) {
     return fail(MMR_HIP_ERROR, "copy of store %lld to host memory failed: %s", (long long)store->id, hipGetErrorString(e));
   }
   store->host = host;
-  ctx->store_epoch += 1;
+  ctx->store_epoch += store->watched;
   ctx->buffer_cache[store->shape_key].push_back(CachedBuffer{store->base, store->bytes});
   store->base = nullptr;
   return MMR_OK;
@@ -1781,7 +1783,7 @@ int mmr_store_reload(mmr_context* ctx, mmr_store* store) {
     return fail(MMR_HIP_ERROR, "copy of store %lld back to the device failed: %s", (long long)store->id, hipGetErrorString(e));
   }
   store->base = base;
-  ctx->store_epoch += 1;
+  ctx->store_epoch += store->watched;
   // the pinned buffer goes to the host cache at once: the next offload into it is ordered behind this copy
   ctx->host_cache[store->shape_key].push_back(CachedBuffer{store->host, store->bytes});
   store->host = nullptr;

@@ -43,8 +43,9 @@ int context_upload(mmr_context* ctx, void* device, const void* host, size_t byte
 void context_attach(mmr_context* ctx, std::unique_ptr<Attachment> a);
 void context_detach(mmr_context* ctx, Attachment* a);  // destroys it
 
-// Counts what may change where a store's buffers are: frees, offloads, reloads.
+// Counts what may change where the buffers of watched stores are: frees, offloads, reloads.
 uint64_t context_store_epoch(mmr_context* ctx);
+void context_watch(mmr_store* store);
 mmr_store* context_find_store(mmr_context* ctx, int64_t id);  // null if it was freed
 // The store is this context's and on the device.
 int context_check_store(mmr_context* ctx, const mmr_store* store, const char* what);

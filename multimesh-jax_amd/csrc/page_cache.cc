@@ -308,6 +308,8 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
                    static_cast<uint32_t>(chunks), mmr::make_fastdiv(static_cast<uint32_t>(chunks))};
   p->move.aligned = aligned;
   p->table_id = mmr_store_id(table), p->lengths_id = mmr_store_id(lengths), p->refs_id = mmr_store_id(refs);
+  for (int32_t i = 0; i < n_pools; ++i) mmr::context_watch(pools[i]);
+  for (mmr_store* t : {table, lengths, refs}) mmr::context_watch(t);
   p->epoch = mmr::context_store_epoch(ctx);
   mmr_pages* handle = p.get();
   mmr::context_attach(ctx, std::move(p));
@@ -335,8 +337,10 @@ int mmr_pages_extend(mmr_pages* pages, const int32_t* sequences, const int32_t* 
   if (int rc = check_ids(tokens, n, "tokens")) return rc;
   if (n == 0) return MMR_OK;
   mmr::context_hash(pages->owner, 16, {static_cast<uint64_t>(n)});
-  MMR_HIP(mmr::launch_page_extend(pages->state, pages->work, sequences, tokens, n, mmr::context_stream(pages->owner)));
-  mmr::context_count(pages->owner, 1);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_extend(pages->state, pages->work, sequences, tokens, n, mmr::context_stream(pages->owner), &launches);
+  mmr::context_count(pages->owner, launches);
+  MMR_HIP(e);
   return MMR_OK;
 } catch (...) {
   return exception_status();
@@ -349,8 +353,10 @@ int mmr_pages_free(mmr_pages* pages, const int32_t* sequences, int32_t n) try {
   if (int rc = check_ids(sequences, n, "sequences")) return rc;
   if (n == 0) return MMR_OK;
   mmr::context_hash(pages->owner, 17, {static_cast<uint64_t>(n)});
-  MMR_HIP(mmr::launch_page_free(pages->state, pages->work, sequences, n, mmr::context_stream(pages->owner)));
-  mmr::context_count(pages->owner, 1);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_free(pages->state, pages->work, sequences, n, mmr::context_stream(pages->owner), &launches);
+  mmr::context_count(pages->owner, launches);
+  MMR_HIP(e);
   return MMR_OK;
 } catch (...) {
   return exception_status();
@@ -364,9 +370,11 @@ int mmr_pages_fork(mmr_pages* pages, const int32_t* parents, const int32_t* chil
   if (int rc = check_ids(children, n, "children")) return rc;
   if (n == 0) return MMR_OK;
   mmr::context_hash(pages->owner, 18, {static_cast<uint64_t>(n)});
-  MMR_HIP(mmr::launch_page_fork(pages->state, pages->work, parents, children, n, moves_up_to(pages, n),
-                                mmr::context_stream(pages->owner)));
-  mmr::context_count(pages->owner, 2);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_fork(pages->state, pages->work, parents, children, n, moves_up_to(pages, n),
+                                mmr::context_stream(pages->owner), &launches);
+  mmr::context_count(pages->owner, launches);
+  MMR_HIP(e);
   return MMR_OK;
 } catch (...) {
   return exception_status();
@@ -377,9 +385,11 @@ int mmr_pages_compact(mmr_pages* pages) try {
   mmr::ContextLock lock(pages->owner);
   if (int rc = begin(pages, 0, 0, "")) return rc;
   mmr::context_hash(pages->owner, 19, {});
-  MMR_HIP(mmr::launch_page_compact(pages->state, pages->work, moves_up_to(pages, pages->state.P / 2),
-                                   mmr::context_stream(pages->owner)));
-  mmr::context_count(pages->owner, 2);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_compact(pages->state, pages->work, moves_up_to(pages, pages->state.P / 2),
+                                   mmr::context_stream(pages->owner), &launches);
+  mmr::context_count(pages->owner, launches);
+  MMR_HIP(e);
   return MMR_OK;
 } catch (...) {
   return exception_status();
@@ -393,9 +403,11 @@ int mmr_pages_copy(mmr_pages* pages, const int32_t* sources, const int32_t* dest
   if (int rc = check_ids(destinations, n, "destinations")) return rc;
   if (n == 0) return MMR_OK;
   mmr::context_hash(pages->owner, 20, {static_cast<uint64_t>(n)});
-  MMR_HIP(mmr::launch_page_copy(pages->state, pages->work, sources, destinations, n, moves_up_to(pages, n),
-                                mmr::context_stream(pages->owner)));
-  mmr::context_count(pages->owner, 2);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_copy(pages->state, pages->work, sources, destinations, n, moves_up_to(pages, n),
+                                mmr::context_stream(pages->owner), &launches);
+  mmr::context_count(pages->owner, launches);
+  MMR_HIP(e);
   return MMR_OK;
 } catch (...) {
   return exception_status();
@@ -408,8 +420,10 @@ int mmr_pages_status(mmr_pages* pages, uint32_t* flags, int64_t* pages_in_use) t
   if (int rc = begin(pages, 0, 0, "")) return rc;
   if (int rc = mmr::context_refuse_capture(ctx, "reading the status of a page cache")) return rc;
   hipStream_t stream = mmr::context_stream(ctx);
-  MMR_HIP(mmr::launch_page_count(pages->state, pages->work, stream));
-  mmr::context_count(ctx, 1);
+  int launches = 0;
+  const hipError_t e = mmr::launch_page_count(pages->state, pages->work, stream, &launches);
+  mmr::context_count(ctx, launches);
+  MMR_HIP(e);
   int32_t header[8] = {};
   MMR_HIP(hipMemcpyAsync(header, pages->work.header, sizeof(header), hipMemcpyDeviceToHost, stream));
   MMR_HIP(hipMemsetAsync(pages->work.header + mmr::kPageStatus, 0, 4, stream));

@@ -22,15 +22,16 @@ struct PageMoveLaunch {
   bool aligned;  // every page is a multiple of 16 bytes
 };
 
+// All of them add the launches they make to *launches.
 hipError_t launch_page_extend(const PageState& st, const PageWork& w, const int32_t* slots, const int32_t* counts, int32_t n,
-                              hipStream_t stream);
-hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_t* slots, int32_t n, hipStream_t stream);
+                              hipStream_t stream, int* launches);
+hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_t* slots, int32_t n, hipStream_t stream, int* launches);
 hipError_t launch_page_fork(const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children, int32_t n,
-                            const PageMoveLaunch& mv, hipStream_t stream);
-hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream);
+                            const PageMoveLaunch& mv, hipStream_t stream, int* launches);
+hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream, int* launches);
 hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
-                            const PageMoveLaunch& mv, hipStream_t stream);
-hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream);
+                            const PageMoveLaunch& mv, hipStream_t stream, int* launches);
+hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream, int* launches);
 
 // One call's rows: at most kRotaryShapes shapes, any number of buffers (several launches if there are many).
 struct RotaryLaunch {

@@ -243,11 +243,16 @@ hipError_t launch_rotary_part(const RotaryLaunch& l, size_t at, int n, hipStream
   return launch_rotary_args(l, args, blocks, n, stream);
 }
 
+hipError_t launched(int* launches) {
+  *launches += 1;
+  return hipGetLastError();
+}
+
 // The launch before a plan, where the pool is more than a plan scans itself.
-hipError_t launch_scan(const PageState& st, const PageWork& w, bool live, hipStream_t stream) {
+hipError_t launch_scan(const PageState& st, const PageWork& w, bool live, hipStream_t stream, int* launches) {
   if (w.n_segments <= kPlanScans) return hipSuccess;
   hipLaunchKernelGGL(mmr_page_scan_kernel, dim3(static_cast<uint32_t>(w.n_segments)), dim3(kPagePlanThreads), 0, stream, st, w, live);
-  return hipGetLastError();
+  return launched(launches);
 }
 
 // Workgroups of a move: one per chunk up to this many, which then loop.
@@ -262,7 +267,7 @@ constexpr uint64_t kFewChunks = 256;
 
 template <int KIND>
 hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
-                        const int32_t* children, int32_t n, uint32_t row_blocks, hipStream_t stream) {
+                        const int32_t* children, int32_t n, uint32_t row_blocks, hipStream_t stream, int* launches) {
   const uint64_t items = static_cast<uint64_t>(mv.max_moves) * mv.mover.n_buffers * mv.mover.chunks;
   const uint32_t movers = static_cast<uint32_t>(items < kMaxMoveBlocks ? (items + 511) / 512 * 512 : kMaxMoveBlocks);
   if (movers + row_blocks == 0) return hipSuccess;
@@ -272,7 +277,7 @@ hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLa
   else
     hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, false>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
                        mv.mover, parents, children, n, row_blocks);
-  return hipGetLastError();
+  return launched(launches);
 }
 
 }  // namespace
@@ -283,65 +288,65 @@ hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLa
 constexpr int64_t kExtendWhole = 16384;
 
 hipError_t launch_page_extend(const PageState& st, const PageWork& w, const int32_t* slots, const int32_t* counts, int32_t n,
-                              hipStream_t stream) {
+                              hipStream_t stream, int* launches) {
   const int64_t most = static_cast<int64_t>(n) * st.B;
   const bool whole = (most < st.P ? most : st.P) <= kExtendWhole;
-  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+  if (hipError_t e = launch_scan(st, w, false, stream, launches)) return e;
   hipLaunchKernelGGL(mmr_page_extend_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, slots, counts, n, whole);
-  if (hipError_t e = hipGetLastError()) return e;
+  if (hipError_t e = launched(launches)) return e;
   if (whole) return hipSuccess;
   hipLaunchKernelGGL(mmr_page_extend_rows_kernel, dim3(static_cast<uint32_t>(n < 4096 ? n : 4096)), dim3(kPageThreads), 0, stream, st,
                      w, slots, counts, n);
-  return hipGetLastError();
+  return launched(launches);
 }
 
-hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_t* slots, int32_t n, hipStream_t stream) {
+hipError_t launch_page_free(const PageState& st, const PageWork& w, const int32_t* slots, int32_t n, hipStream_t stream, int* launches) {
   hipLaunchKernelGGL(mmr_page_free_kernel, dim3(static_cast<uint32_t>(n)), dim3(kPagePlanThreads), 0, stream, st, w, slots);
-  return hipGetLastError();
+  return launched(launches);
 }
 
 hipError_t launch_page_fork(const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children, int32_t n,
-                            const PageMoveLaunch& mv, hipStream_t stream) {
-  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+                            const PageMoveLaunch& mv, hipStream_t stream, int* launches) {
+  if (hipError_t e = launch_scan(st, w, false, stream, launches)) return e;
   hipLaunchKernelGGL(mmr_page_fork_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, parents, children, n);
-  if (hipError_t e = hipGetLastError()) return e;
-  return launch_apply<1>(st, w, mv, parents, children, n, static_cast<uint32_t>(n < 4096 ? n : 4096), stream);
+  if (hipError_t e = launched(launches)) return e;
+  return launch_apply<1>(st, w, mv, parents, children, n, static_cast<uint32_t>(n < 4096 ? n : 4096), stream, launches);
 }
 
-hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream) {
+hipError_t launch_page_compact(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, hipStream_t stream, int* launches) {
   const bool whole = st.P <= kCompactWhole;
-  if (hipError_t e = launch_scan(st, w, true, stream)) return e;
+  if (hipError_t e = launch_scan(st, w, true, stream, launches)) return e;
   hipLaunchKernelGGL(mmr_page_compact_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, whole);
-  if (hipError_t e = hipGetLastError()) return e;
+  if (hipError_t e = launched(launches)) return e;
   if (!whole) {
     const uint32_t blocks = (mv.max_moves + kPageThreads - 1) / kPageThreads;
     hipLaunchKernelGGL(mmr_page_compact_list_kernel, dim3(blocks < 1024 ? blocks : 1024), dim3(kPageThreads), 0, stream, st, w);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = launched(launches)) return e;
   }
-  return launch_apply<2>(st, w, mv, nullptr, nullptr, 0, static_cast<uint32_t>(st.S < 4096 ? st.S : 4096), stream);
+  return launch_apply<2>(st, w, mv, nullptr, nullptr, 0, static_cast<uint32_t>(st.S < 4096 ? st.S : 4096), stream, launches);
 }
 
 hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
-                            const PageMoveLaunch& mv, hipStream_t stream) {
+                            const PageMoveLaunch& mv, hipStream_t stream, int* launches) {
   const uint64_t items = static_cast<uint64_t>(n) * mv.mover.n_buffers * mv.mover.chunks;
   if (n <= kFewPairs && items <= kFewChunks) {
     const dim3 grid(static_cast<uint32_t>(items));
     if (mv.aligned) hipLaunchKernelGGL(mmr_page_copy_few_kernel<true>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
     else hipLaunchKernelGGL(mmr_page_copy_few_kernel<false>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
-    return hipGetLastError();
+    return launched(launches);
   }
   // in the order of the destinations 512 pages of 32 KiB in each of 48 buffers take 293 us, in the caller's 308; where the pairs
   // are few among the pages the pass over these costs more than it gives (512 of 20,000: 59 us, sorted 69)
   const bool sorted = st.P / 8 <= n;
   hipLaunchKernelGGL(mmr_page_copy_plan_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w, src, dst, n, sorted);
-  if (hipError_t e = hipGetLastError()) return e;
-  return launch_apply<0>(st, w, mv, nullptr, nullptr, 0, 0, stream);
+  if (hipError_t e = launched(launches)) return e;
+  return launch_apply<0>(st, w, mv, nullptr, nullptr, 0, 0, stream, launches);
 }
 
-hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream) {
-  if (hipError_t e = launch_scan(st, w, false, stream)) return e;
+hipError_t launch_page_count(const PageState& st, const PageWork& w, hipStream_t stream, int* launches) {
+  if (hipError_t e = launch_scan(st, w, false, stream, launches)) return e;
   hipLaunchKernelGGL(mmr_page_count_kernel, dim3(1), dim3(kPagePlanThreads), 0, stream, st, w);
-  return hipGetLastError();
+  return launched(launches);
 }
 
 hipError_t launch_rotary(const RotaryLaunch& l, int* launches, hipStream_t stream) {

@@ -114,8 +114,8 @@ MMR_HD void page_plan_scan(X& x, const PageState& st, const PageWork& w, bool li
   x.sync();
 }
 
-// The free pages of all segments, once every segment is scanned: in the plan's last workgroup, or (`counted`) in a later
-// launch.
+// The free pages of all segments, once every segment is scanned: summed by the plan, or taken from what the plan
+// published (`counted`).
 template <class X, int32_t kSegment = kPagesPerThread * X::kThreads>
 struct FreePages {
   const PageWork* w;

@@ -265,7 +265,8 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
   if (j.paged) {
     // the token of the wave's first lane, for all lanes to look up together
     const uint32_t first = small_div(small_div(static_cast<uint32_t>(x.tid) & ~63u, j.mul_lanes), j.mul_head_lanes);
-    const int32_t wave_token = static_cast<int32_t>(group * j.token_lanes + first);
+    const uint32_t ask = group * j.token_lanes + first;
+    const int32_t wave_token = static_cast<int32_t>(ask < j.tokens ? ask : j.tokens - 1);
     int32_t page = 0, in_page = 0;
     uint32_t bad = 0;
     // lanes without a token ask for their wave's first one and go no further
