@@ -178,11 +178,6 @@ int check_rotary(mmr_context* ctx, const mmr_rotary* r, int64_t dim, int32_t dty
   return MMR_OK;
 }
 
-// Whole 16-byte vectors throughout: the rotated part (its two halves, unless interleaved), the row and every stride.
-bool vector_rows(int64_t rotated, bool interleaved, int64_t dim, int itemsize) {
-  return ((interleaved ? rotated : rotated / 2) * itemsize) % 16 == 0 && (dim * itemsize) % 16 == 0;
-}
-
 constexpr uint64_t kMaxRotaryBlocks = (1u << 24) - 1;  // a grid has fewer than 2^32 threads
 
 constexpr int64_t kL2Bytes = int64_t{32} << 20;  // eight XCDs of 4 MiB
@@ -194,34 +189,48 @@ void set_plan(mmr::RotaryLaunch* l, const mmr_rotary* r, bool backward) {
   l->interleaved = r->interleaved;
 }
 
-// What of a row a launch does: its length in elements, and whether it is turned and in place (then the rest of it stays).
+// What of a row a call does: its length in elements, and whether it is turned and in place.
 struct Row {
   int64_t dim;
   bool turned, in_place;
 };
 
+// Bytes of the vectors a lane turns: 16 where every row, its turned part (its two halves, unless interleaved) and with
+// them every stride are whole vectors, else the widest that divides the turned part - these may stand at any address.
+int vector_bytes(const mmr::RotaryLaunch& l, const std::vector<Row>& rows, int itemsize) {
+  const int64_t part = static_cast<int64_t>(l.angles.half) * itemsize * (l.interleaved ? 2 : 1);
+  bool wide = true, turned = false;
+  for (const Row& r : rows) {
+    wide &= r.dim * itemsize % 16 == 0;
+    turned |= r.turned;
+  }
+  if (!turned) return wide ? 16 : 1;
+  if (wide && part % 16 == 0) return 16;
+  for (int bytes = 8; bytes > itemsize; bytes /= 2)
+    if (part % bytes == 0) return bytes;
+  return itemsize;
+}
+
 // Units of the shapes, and the launches.  A call of few rows takes one head a lane, so that its latency is one row's and
 // not four.
 int launch_rows(mmr_context* ctx, mmr::RotaryLaunch* l, const std::vector<Row>& rows, int itemsize) {
-  const int64_t vec = l->type < 0 ? (l->vectors ? 16 : 1) : (l->vectors ? 16 / itemsize : 1);
-  const int64_t per = l->type < 0 ? itemsize : 1;  // raw rows are counted in bytes
-  int64_t lanes = 0, bytes = 0;
-  std::vector<std::pair<uint32_t, uint32_t>> units;
-  for (const Row& r : rows) {
-    const int64_t rot = r.turned ? static_cast<int64_t>(l->angles.half) : 0;
-    const int64_t rest = r.in_place ? 0 : r.dim * per - 2 * rot;
-    const bool one = l->interleaved && l->vectors;  // a unit is one vector, not two
-    units.push_back({static_cast<uint32_t>((one ? 2 * rot : rot) / vec), static_cast<uint32_t>(rest / vec)});
+  l->vector_bytes = vector_bytes(*l, rows, itemsize);
+  for (size_t i = 0; i < rows.size(); ++i) {
+    const int64_t turned = rows[i].turned ? static_cast<int64_t>(l->angles.half) * 2 * itemsize : 0;
+    const int64_t unit = static_cast<int64_t>(l->vector_bytes) * (l->interleaved ? 1 : 2);
+    mmr::rotary_units(&l->shapes[i], static_cast<uint32_t>(rows[i].dim * itemsize), static_cast<uint32_t>(turned),
+                      static_cast<uint32_t>(unit), static_cast<uint32_t>(l->type < 0 ? 1 : itemsize), rows[i].in_place);
   }
+  int64_t lanes = 0, bytes = 0;
   for (const mmr::RotaryBuffer& b : l->buffers) {
     const int64_t n = static_cast<int64_t>(b.outer) * b.seq * b.heads;
-    lanes += n * (units[b.shape].first + units[b.shape].second);
+    lanes += n * l->shapes[b.shape].units;
     bytes += n * rows[b.shape].dim * itemsize;
   }
   const bool spread = lanes < 256 * 1024;  // a lane each would leave the 256 CUs under four workgroups
   for (size_t i = 0; i < l->shapes.size(); ++i) {
     mmr::RotaryShape& j = l->shapes[i];
-    if (mmr::rotary_shape(&j, units[i].first, units[i].second, j.src_head <= j.src_seq, spread) > kMaxRotaryBlocks)
+    if (mmr::rotary_shape(&j, j.src_head <= j.src_seq, spread) > kMaxRotaryBlocks)
       return fail(MMR_UNSUPPORTED, "a tile of %u tokens of %u heads is more than a launch takes", j.tokens, j.heads);
   }
   l->past_caches = bytes > kL2Bytes;
@@ -305,8 +314,10 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
               reinterpret_cast<int32_t*>(mmr::store_tile(refs, 0)), static_cast<int32_t>(S), static_cast<int32_t>(B),
               static_cast<int32_t>(P), page_tokens, static_cast<int32_t>(capacity), mmr::make_fastdiv(static_cast<uint32_t>(page_tokens))};
   p->move.mover = {reinterpret_cast<const mmr::PageBuffer*>(p->block + p->buffers_at), static_cast<uint32_t>(buffers),
-                   static_cast<uint32_t>(chunks), mmr::make_fastdiv(static_cast<uint32_t>(chunks))};
+                   static_cast<uint32_t>(chunks), mmr::make_fastdiv(static_cast<uint32_t>(chunks)),
+                   mmr::page_lane_bits(static_cast<uint64_t>(largest))};
   p->move.aligned = aligned;
+  p->move.packed = (1 << p->move.mover.lane_bits) < mmr::kPageThreads;
   p->table_id = mmr_store_id(table), p->lengths_id = mmr_store_id(lengths), p->refs_id = mmr_store_id(refs);
   for (int32_t i = 0; i < n_pools; ++i) mmr::context_watch(pools[i]);
   for (mmr_store* t : {table, lengths, refs}) mmr::context_watch(t);
@@ -540,7 +551,6 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
   mmr::RotaryLaunch l;
   set_plan(&l, rotary, flags & MMR_ROTARY_BACKWARD);
   l.type = s.dtype;
-  l.vectors = vector_rows(rotary->dim, rotary->interleaved, s.size[s.rank - 1], s.itemsize);
   const int64_t all_outer = outer >= 0 ? s.ext[outer] : 1, all_heads = head >= 0 ? s.ext[head] : 1, all_seq = s.ext[seq_dim];
   if (all_outer == 0 || all_heads == 0 || all_seq == 0) return MMR_OK;  // an empty array
   if (all_outer > 0x7fffffff / all_seq || all_heads > 0x7fffffff) return fail(MMR_UNSUPPORTED, "a tile of more than 2^31 rows");
@@ -608,7 +618,6 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
   int64_t tokens = -1;
   int32_t dtype = -1;
   int itemsize = 0;
-  bool vectors = true;
   // a new-token store: [tokens, heads, dim], tokens unsharded, every part of one call of the same type and length
   auto check_new = [&](const mmr_store* s, const char* what) {
     if (int rc = mmr::context_check_store(ctx, s, what)) return rc;
@@ -650,7 +659,6 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
     }
     l.shapes.push_back(j);
     rows.push_back(Row{d.size[2], turn, in_place});
-    vectors &= vector_rows(turn ? rotary->dim : 0, l.interleaved, d.size[2], d.itemsize);
   };
   auto add_pool = [&](const mmr_store* s, int32_t pool, bool turn, const char* what) {
     if (int rc = check_new(s, what)) return rc;
@@ -685,7 +693,6 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
     if (int rc = add_pool(v, v_pool, false, "v")) return rc;
   if (n == 0 || l.buffers.empty()) return MMR_OK;
   l.type = rotary ? dtype : -1;
-  l.vectors = vectors;
   const mmr::PageState& st = pages->state;
   l.pages = {st.table, st.lengths, sequences, begins, pages->work.header + mmr::kPageStatus, n, st.S, st.B, st.P, st.T,
                   st.capacity, st.div_T};

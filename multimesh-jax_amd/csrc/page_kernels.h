@@ -20,6 +20,7 @@ struct PageMoveLaunch {
   PageMover mover;
   uint32_t max_moves;
   bool aligned;  // every page is a multiple of 16 bytes
+  bool packed;   // a page takes at most half a workgroup, 16 bytes a lane
 };
 
 // All of them add the launches they make to *launches.
@@ -40,8 +41,9 @@ struct RotaryLaunch {
   std::vector<RotaryShape> shapes;
   std::vector<RotaryBuffer> buffers;
   int type = -1;  // MMR_F32, MMR_BF16 or MMR_F16; -1: rows only move (nothing is turned)
-  bool vectors = false, interleaved = false;
-  bool past_caches = false;  // how results are stored
+  int vector_bytes = 0;  // 16: rows, turned parts and strides are whole vectors; else what divides the turned part
+  bool interleaved = false;
+  bool past_caches = false;  // how results are stored (16-byte vectors alone)
 };
 hipError_t launch_rotary(const RotaryLaunch& l, int* launches, hipStream_t stream);
 

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_copy_few_kernel(PageSta
   __shared__ int32_t pairs[2 * kFewPairs];
   ApplyGroup x(scan);
   if (!page_copy_few(x, st, w, pairs, src, dst, n)) return;
-  page_move_chunk<StreamMem, ALIGNED>(mv, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; },
+  page_move_chunk<StreamMem, ALIGNED, false>(mv, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; },
                                       static_cast<uint32_t>(n), blockIdx.x, threadIdx.x);
 }
 
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kPagePlanThreads) void mmr_page_free_kernel(PageSta
 // a fork copies is often the last one of several entries: its loads go through the caches (256 sequences forked from 16,
 // 402 MB written: 82 us; past the caches 131 us).  A copy or a compact reads every page once, past the caches (copy of
 // 805 MB 308 us, through them 311; compact 719 and 728).
-template <int KIND, bool ALIGNED>
+template <int KIND, bool ALIGNED, bool PACKED>
 __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState st, PageWork w, PageMover mv,
                                                                       const int32_t* parents, const int32_t* children, int32_t n,
                                                                       uint32_t row_blocks) {
@@ -177,12 +177,12 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState 
     else page_compact_rows(x, st, w, blockIdx.x, row_blocks);
     return;
   }
-  const uint32_t moves = static_cast<uint32_t>(w.header[kPageMoves]), items = moves * mv.n_buffers * mv.chunks;
+  const uint32_t moves = static_cast<uint32_t>(w.header[kPageMoves]), items = page_items<PACKED>(mv, moves);
   const uint32_t step = gridDim.x - row_blocks;
   for (uint32_t at = blockIdx.x - row_blocks; at < (items + 511u) / 512u * 512u; at += step) {
     const uint32_t item = chunk_index(at, 64);  // runs of 64 neighbours share an XCD
     typedef DeviceMem<KIND != 1, true> M;
-    if (item < items) page_move_chunk<M, ALIGNED>(mv, [&](uint32_t i) { return w.moves[i]; }, moves, item, threadIdx.x);
+    if (item < items) page_move_chunk<M, ALIGNED, PACKED>(mv, [&](uint32_t i) { return w.moves[i]; }, moves, item, threadIdx.x);
   }
 }
 
@@ -201,27 +201,39 @@ __global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(Args a) {
 template <class Args>
 hipError_t launch_rotary_args(const RotaryLaunch& l, const Args& args, uint32_t blocks, int n, hipStream_t stream) {
   const dim3 grid(blocks, static_cast<uint32_t>(n)), threads(kRotaryThreads);
-#define MMR_ROTARY(T, V, I)                                                                                           \
-  do {                                                                                                               \
-    if (l.past_caches) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, true, Args>), grid, threads, 0, stream, args);    \
-    else hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, false, Args>), grid, threads, 0, stream, args);                 \
+#define MMR_ROTARY(T, V, I, S) hipLaunchKernelGGL((mmr_rotary_kernel<T, V, I, S, Args>), grid, threads, 0, stream, args)
+#define MMR_ROTARY_WIDE(T, V, I)                      \
+  do {                                                \
+    if (l.past_caches) MMR_ROTARY(T, V, I, true);     \
+    else MMR_ROTARY(T, V, I, false);                  \
   } while (0)
-#define MMR_ROTARY_TYPE(T, V)                                       \
-  do {                                                              \
-    if (l.vectors && l.interleaved) MMR_ROTARY(T, V, true);         \
-    else if (l.vectors) MMR_ROTARY(T, V, false);                    \
-    else if (l.interleaved) MMR_ROTARY(T, 1, true);                 \
-    else MMR_ROTARY(T, 1, false);                                   \
+// narrower vectors: 8 bytes, 4 bytes, or a single element where the halves of the rotated part are of odd length
+#define MMR_ROTARY_16(T)                                                          \
+  do {                                                                            \
+    if (l.vector_bytes == 16 && l.interleaved) MMR_ROTARY_WIDE(T, 8, true);       \
+    else if (l.vector_bytes == 16) MMR_ROTARY_WIDE(T, 8, false);                  \
+    else if (l.vector_bytes == 8 && l.interleaved) MMR_ROTARY(T, 4, true, false); \
+    else if (l.vector_bytes == 8) MMR_ROTARY(T, 4, false, false);                 \
+    else if (l.interleaved) MMR_ROTARY(T, 2, true, false);                        \
+    else if (l.vector_bytes == 4) MMR_ROTARY(T, 2, false, false);                 \
+    else MMR_ROTARY(T, 1, false, false);                                          \
   } while (0)
   switch (l.type) {
-    case MMR_F32: MMR_ROTARY_TYPE(RotaryF32, 4); break;
-    case MMR_BF16: MMR_ROTARY_TYPE(RotaryBF16, 8); break;
-    case MMR_F16: MMR_ROTARY_TYPE(RotaryF16, 8); break;
+    case MMR_F32:
+      if (l.vector_bytes == 16 && l.interleaved) MMR_ROTARY_WIDE(RotaryF32, 4, true);
+      else if (l.vector_bytes == 16) MMR_ROTARY_WIDE(RotaryF32, 4, false);
+      else if (l.interleaved) MMR_ROTARY(RotaryF32, 2, true, false);
+      else if (l.vector_bytes == 8) MMR_ROTARY(RotaryF32, 2, false, false);
+      else MMR_ROTARY(RotaryF32, 1, false, false);
+      break;
+    case MMR_BF16: MMR_ROTARY_16(RotaryBF16); break;
+    case MMR_F16: MMR_ROTARY_16(RotaryF16); break;
     default:
-      if (l.vectors) MMR_ROTARY(RotaryRaw, 16, false);
-      else MMR_ROTARY(RotaryRaw, 1, false);
+      if (l.vector_bytes == 16) MMR_ROTARY_WIDE(RotaryRaw, 16, false);
+      else MMR_ROTARY(RotaryRaw, 1, false, false);
   }
-#undef MMR_ROTARY_TYPE
+#undef MMR_ROTARY_16
+#undef MMR_ROTARY_WIDE
 #undef MMR_ROTARY
   return hipGetLastError();
 }
@@ -268,15 +280,17 @@ constexpr uint64_t kFewChunks = 256;
 template <int KIND>
 hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
                         const int32_t* children, int32_t n, uint32_t row_blocks, hipStream_t stream, int* launches) {
-  const uint64_t items = static_cast<uint64_t>(mv.max_moves) * mv.mover.n_buffers * mv.mover.chunks;
+  const uint64_t items = mv.packed ? page_items<true>(mv.mover, mv.max_moves) : page_items<false>(mv.mover, mv.max_moves);
   const uint32_t movers = static_cast<uint32_t>(items < kMaxMoveBlocks ? (items + 511) / 512 * 512 : kMaxMoveBlocks);
   if (movers + row_blocks == 0) return hipSuccess;
-  if (mv.aligned)
-    hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, true>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
-                       mv.mover, parents, children, n, row_blocks);
-  else
-    hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, false>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w,
-                       mv.mover, parents, children, n, row_blocks);
+#define MMR_APPLY(A, P)                                                                                                          \
+  hipLaunchKernelGGL((mmr_page_apply_kernel<KIND, A, P>), dim3(movers + row_blocks), dim3(kPageThreads), 0, stream, st, w, mv.mover, \
+                     parents, children, n, row_blocks)
+  if (mv.aligned && mv.packed) MMR_APPLY(true, true);
+  else if (mv.aligned) MMR_APPLY(true, false);
+  else if (mv.packed) MMR_APPLY(false, true);
+  else MMR_APPLY(false, false);
+#undef MMR_APPLY
   return launched(launches);
 }
 

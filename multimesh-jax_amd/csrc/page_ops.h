@@ -72,6 +72,7 @@ struct PageMover {
   uint32_t n_buffers;
   uint32_t chunks;  // chunks of kPageChunkBytes in the largest page
   FastDiv div_chunks;
+  uint32_t lane_bits;  // page_lane_bits
 };
 
 constexpr uint32_t kPageChunkBytes = 8192;
@@ -530,15 +531,41 @@ MMR_HD void page_count(X& x, const PageState& st, const PageWork& w, int32_t* sh
   if (x.tid == 0) w.header[kPageLive] = st.P - pages.total;
 }
 
-// Chunk `item` of the moves, buffer after buffer, move after move: the pages of one buffer are worked off together, so
+// Lanes that share a page of at most a chunk, where a workgroup moves several: a power of two.
+inline uint32_t page_lane_bits(uint64_t largest) {
+  uint32_t bits = 0;
+  const uint64_t lanes = (largest + 15) / 16;
+  while ((1u << bits) < static_cast<uint32_t>(kPageThreads) && (1u << bits) < lanes) ++bits;
+  return bits;
+}
+
+// Items of a launch: chunks of pages, or, PACKED, groups of pages that a workgroup moves together.
+template <bool PACKED>
+MMR_HD uint32_t page_items(const PageMover& m, uint32_t n_moves) {
+  if (!PACKED) return n_moves * m.n_buffers * m.chunks;
+  const uint32_t together = static_cast<uint32_t>(kPageThreads) >> m.lane_bits;
+  return (n_moves + together - 1) / together * m.n_buffers;
+}
+
+// Item `item` of the moves, buffer after buffer, move after move: the pages of one buffer are worked off together, so
 // that the workgroups in flight share their address translations.  move(i): move i.  M: memory policy of chunk_ops.h.
 // Pages of a multiple of 16 bytes move as aligned 16-byte vectors.  Others move as 16-byte vectors at any alignment, the
 // last one slid back to end with the page (it repeats bytes of its neighbour, with the same values), pages under 16 bytes
-// byte by byte.
-template <class M, bool ALIGNED, class Move>
-MMR_HD void page_move_chunk(const PageMover& m, Move move, uint32_t n_moves, uint32_t item, uint32_t tid) {
-  const uint32_t rest = fdiv(item, m.div_chunks), chunk = item - rest * m.chunks;
-  const uint32_t bi = rest / n_moves, mi = rest - bi * n_moves;
+// byte by byte.  PACKED (no page longer than 16 bytes a lane): 2^lane_bits lanes a page.
+template <class M, bool ALIGNED, bool PACKED, class Move>
+MMR_HD void page_move_chunk(const PageMover& m, Move move, uint32_t n_moves, uint32_t item, uint32_t thread) {
+  uint32_t bi, mi, chunk = 0, tid = thread;
+  if (PACKED) {
+    const uint32_t together = static_cast<uint32_t>(kPageThreads) >> m.lane_bits, groups = (n_moves + together - 1) / together;
+    bi = item / groups;
+    mi = (item - bi * groups) * together + (thread >> m.lane_bits);
+    tid = thread & ((1u << m.lane_bits) - 1);
+    if (mi >= n_moves) return;
+  } else {
+    const uint32_t rest = fdiv(item, m.div_chunks);
+    chunk = item - rest * m.chunks;
+    bi = rest / n_moves, mi = rest - bi * n_moves;
+  }
   const PageBuffer b = m.buffers[bi];
   const PageMove mv = move(mi);
   if (mv.src == mv.dst) return;
@@ -548,7 +575,7 @@ MMR_HD void page_move_chunk(const PageMover& m, Move move, uint32_t n_moves, uin
   const uint32_t bytes = left < kPageChunkBytes ? static_cast<uint32_t>(left) : kPageChunkBytes;
   typename M::cptr s = M::cplace(b.base + static_cast<uint64_t>(mv.src) * b.page_bytes + begin);
   typename M::ptr d = M::place(b.base + static_cast<uint64_t>(mv.dst) * b.page_bytes + begin);
-  constexpr uint32_t kUnroll = kPageChunkBytes / 16 / kPageThreads;
+  constexpr uint32_t kUnroll = PACKED ? 1 : kPageChunkBytes / 16 / kPageThreads;
   if (ALIGNED) {
     V16 v[kUnroll];
 #pragma unroll
@@ -564,7 +591,9 @@ MMR_HD void page_move_chunk(const PageMover& m, Move move, uint32_t n_moves, uin
     return;
   }
   if (b.page_bytes < 16) {
-    if (tid < bytes) M::template storeu<uint8_t>(d + tid, M::template loadu<uint8_t>(s + tid));
+    // a larger page of another pool may have set few lanes
+    for (uint32_t at = tid; at < bytes; at += PACKED ? 1u << m.lane_bits : static_cast<uint32_t>(kPageThreads))
+      M::template storeu<uint8_t>(d + at, M::template loadu<uint8_t>(s + at));
     return;
   }
   // the last vector of a page may reach back into the chunk before: begin > 0 or the page holds 16 bytes here

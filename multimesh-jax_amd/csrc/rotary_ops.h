@@ -38,6 +38,7 @@ struct RotaryShape {
   int64_t pos_outer, pos_seq;            // in elements
   uint32_t tokens, seq, heads;           // tokens = outer * seq
   uint32_t rot_units, units;             // units of a row: rotated ones first
+  uint32_t rest_at, rest_bytes;          // the part that passes through
   uint32_t head_groups;                  // workgroups along the heads
   uint32_t blocks;                       // workgroups of a buffer
   uint32_t mul_lanes, mul_head_lanes;    // small_div by the two
@@ -133,7 +134,7 @@ struct RotaryF16 {
   static MMR_HD uint32_t put(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
 };
 
-// The 16-byte (or one-element) vector a lane holds, as 32-bit words.
+// The vector of VEC elements a lane turns, as 32-bit words.  Of 16 bytes it is aligned, narrower ones stand anywhere.
 template <class T, int VEC>
 struct RotaryVec {
   static constexpr int kBytes = VEC * T::kBytes;
@@ -145,6 +146,9 @@ struct RotaryVec {
     if constexpr (kBytes == 16) {
       const V16 v = M::load16(p);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint64_t v = M::template loadu<uint64_t>(p);
+      w[0] = static_cast<uint32_t>(v), w[1] = static_cast<uint32_t>(v >> 32);
     } else if constexpr (kBytes == 4) {
       w[0] = M::template loadu<uint32_t>(p);
     } else if constexpr (kBytes == 2) {
@@ -156,6 +160,7 @@ struct RotaryVec {
   template <class M>
   MMR_HD void store(typename M::ptr p) const {
     if constexpr (kBytes == 16) M::store16(p, V16{w[0], w[1], w[2], w[3]});
+    else if constexpr (kBytes == 8) M::template storeu<uint64_t>(p, w[0] | static_cast<uint64_t>(w[1]) << 32);
     else if constexpr (kBytes == 4) M::template storeu<uint32_t>(p, w[0]);
     else if constexpr (kBytes == 2) M::template storeu<uint16_t>(p, static_cast<uint16_t>(w[0]));
     else M::template storeu<uint8_t>(p, static_cast<uint8_t>(w[0]));
@@ -211,13 +216,16 @@ MMR_HD bool rotary_place(X& x, const RotaryPages& pg, int32_t wave_token, int32_
 }
 
 // Lane (row, unit) of workgroup `block` of a buffer.  A unit is what a lane turns: the two vectors that hold VEC pairs, or,
-// interleaved, one vector of VEC / 2 pairs; in the rest of the row it is one vector.  The rows are loaded before the
-// position is looked up: the look-up is a chain of four loads.
+// interleaved, one vector of VEC / 2 pairs; in the rest of the row it is 16 bytes, the last ones slid back to end with the
+// row (they repeat their neighbour's bytes, with the same values), or one element if the rest is shorter.  The rows are
+// loaded before the position is looked up: the look-up is a chain of four loads.
 template <class M, class T, int VEC, bool INTERLEAVED, class X>
 MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, const RotaryShape& j, const RotaryBuffer& b) {
   constexpr int kVecBytes = VEC * T::kBytes;
-  constexpr bool kTwo = T::kBytes > 1 && (!INTERLEAVED || VEC == 1);  // a unit of the rotated part is two vectors
-  constexpr int kPairs = INTERLEAVED && VEC > 1 ? VEC / 2 : VEC;      // and so many pairs
+  static_assert(!INTERLEAVED || VEC > 1, "an interleaved unit holds whole pairs");
+  constexpr bool kTwo = T::kBytes > 1 && !INTERLEAVED;  // a unit of the rotated part is two vectors
+  constexpr int kPairs = INTERLEAVED ? VEC / 2 : VEC;   // and so many pairs
+  constexpr bool kWide = kVecBytes == 16;               // every row and the rest of it are whole aligned vectors
   const uint32_t group = fdiv(x.block, j.div_head_groups), hg = x.block - group * j.head_groups;
   const uint32_t row = small_div(static_cast<uint32_t>(x.tid), j.mul_lanes), lane = static_cast<uint32_t>(x.tid) - row * j.lanes;
   const uint32_t tsub = small_div(row, j.mul_head_lanes), hsub = row - tsub * j.head_lanes;
@@ -230,12 +238,18 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
 
   // byte offsets in a row of the two vectors of a unit (of the one, for units of the rest)
   auto offsets = [&](uint32_t unit, int64_t* off_a, int64_t* off_b) {
-    if (!kTwo || unit >= j.rot_units)
-      *off_a = *off_b = static_cast<int64_t>(unit + (kTwo ? j.rot_units : 0)) * kVecBytes;
-    else if (INTERLEAVED) *off_a = static_cast<int64_t>(2) * unit * kVecBytes, *off_b = *off_a + kVecBytes;
-    else *off_a = static_cast<int64_t>(unit) * kVecBytes, *off_b = *off_a + static_cast<int64_t>(a.half) * T::kBytes;
+    if (unit < j.rot_units) {
+      *off_a = static_cast<int64_t>(unit) * kVecBytes;
+      *off_b = *off_a + static_cast<int64_t>(a.half) * T::kBytes;
+    } else {
+      const uint32_t at = unit - j.rot_units;
+      uint32_t in_rest = at * T::kBytes;
+      if (j.rest_bytes >= 16) in_rest = at * 16 + 16 <= j.rest_bytes ? at * 16 : j.rest_bytes - 16;
+      *off_a = *off_b = static_cast<int64_t>(j.rest_at) + in_rest;
+    }
   };
   RotaryVec<T, VEC> va[kRotaryHeads], vb[kRotaryHeads];
+  V16 rest[kRotaryHeads];  // where the vectors are narrower
   auto load = [&](uint32_t unit) {
     int64_t off_a, off_b;
     offsets(unit, &off_a, &off_b);
@@ -243,7 +257,12 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
     for (uint32_t k = 0; k < kRotaryHeads; ++k) {
       const uint32_t h = h0 + k * j.head_lanes;
       if (k < j.head_steps && h < b.heads) {
-        va[k].template load<M>(M::cplace(src + (h * j.src_head + off_a)));
+        const typename M::cptr from = M::cplace(src + (h * j.src_head + off_a));
+        if (kWide || unit < j.rot_units) va[k].template load<M>(from);
+        else if (j.rest_bytes >= 16) rest[k] = M::load16u(from);
+        else if (T::kBytes == 4) rest[k].x = M::template loadu<uint32_t>(from);
+        else if (T::kBytes == 2) rest[k].x = M::template loadu<uint16_t>(from);
+        else rest[k].x = M::template loadu<uint8_t>(from);
         if (kTwo && unit < j.rot_units) vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
       }
     }
@@ -327,7 +346,13 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
 #pragma unroll
       for (uint32_t k = 0; k < kRotaryHeads; ++k) {
         const uint32_t h = h0 + k * j.head_lanes;
-        if (k < j.head_steps && h < b.heads) va[k].template store<M>(M::place(dst + (h * j.dst_head + off_a)));
+        if (k >= j.head_steps || h >= b.heads) continue;
+        const typename M::ptr to = M::place(dst + (h * j.dst_head + off_a));
+        if (kWide) va[k].template store<M>(to);
+        else if (j.rest_bytes >= 16) M::template storeu<V16>(to, rest[k]);
+        else if (T::kBytes == 4) M::template storeu<uint32_t>(to, rest[k].x);
+        else if (T::kBytes == 2) M::template storeu<uint16_t>(to, static_cast<uint16_t>(rest[k].x));
+        else M::template storeu<uint8_t>(to, static_cast<uint8_t>(rest[k].x));
       }
     }
     unit += j.lanes;
@@ -337,12 +362,18 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
   }
 }
 
+// Units of a row of `bytes` bytes with `turned` of them turned, in units of `unit_bytes`; `element`: bytes of one.
+inline void rotary_units(RotaryShape* j, uint32_t bytes, uint32_t turned, uint32_t unit_bytes, uint32_t element, bool in_place) {
+  j->rot_units = turned / unit_bytes;
+  j->rest_at = turned;
+  j->rest_bytes = in_place ? 0 : bytes - turned;  // in place, what is not turned stays
+  j->units = j->rot_units + (j->rest_bytes >= 16 ? (j->rest_bytes + 15) / 16 : j->rest_bytes / element);
+}
+
 // How the rows of a shape are dealt to workgroups; returns how many that takes.  `spread`: one head a lane, for launches
 // that would not fill the chip.
-inline uint64_t rotary_shape(RotaryShape* j, uint32_t rot_units, uint32_t rest_units, bool heads_adjacent, bool spread) {
+inline uint64_t rotary_shape(RotaryShape* j, bool heads_adjacent, bool spread) {
   const uint32_t threads = kRotaryThreads;
-  j->rot_units = rot_units;
-  j->units = rot_units + rest_units;
   const uint32_t lanes = j->units < threads ? j->units : threads;
   const uint32_t rows = threads / lanes;
   const uint32_t want = spread ? 1u : static_cast<uint32_t>(kRotaryHeads);

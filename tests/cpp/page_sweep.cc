@@ -181,7 +181,7 @@ struct Cache {
     const int32_t capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(B) * T, 0x7fffffff));
     st = {table.p, lengths.p, refs.p, S, B, P, T, capacity, make_fastdiv(static_cast<uint32_t>(T))};
     w = {header.p, seg_free.p, seg_before.p, free_ids.p, live_ids.p, mark.p, len.p, rank.p, moves.p, map.p, segs(p)};
-    mover = {buffers.p, static_cast<uint32_t>(bytes.size()), chunks, make_fastdiv(chunks)};
+    mover = {buffers.p, static_cast<uint32_t>(bytes.size()), chunks, make_fastdiv(chunks), page_lane_bits(largest)};
   }
   static int32_t segs(int32_t p) { return (p + kSegment - 1) / kSegment; }
 
@@ -209,18 +209,21 @@ struct Cache {
     return s;
   }
   template <class Move>
-  void chunk(uint32_t item, uint32_t n, uint32_t tid, Move m) {
-    if (aligned) page_move_chunk<Mem, true>(mover, m, n, item, tid);
-    else page_move_chunk<Mem, false>(mover, m, n, item, tid);
+  void chunk(uint32_t item, uint32_t n, uint32_t tid, Move m, bool packed) {
+    if (aligned && packed) page_move_chunk<Mem, true, true>(mover, m, n, item, tid);
+    else if (aligned) page_move_chunk<Mem, true, false>(mover, m, n, item, tid);
+    else if (packed) page_move_chunk<Mem, false, true>(mover, m, n, item, tid);
+    else page_move_chunk<Mem, false, false>(mover, m, n, item, tid);
   }
   void move(std::mt19937_64& rng) {
     if (!header[kPageOk]) return;
-    const uint32_t items = static_cast<uint32_t>(header[kPageMoves]) * mover.n_buffers * mover.chunks;
+    const bool packed = (1 << mover.lane_bits) < kPageThreads && rng() % 4;
+    const uint32_t n = static_cast<uint32_t>(header[kPageMoves]), items = packed ? page_items<true>(mover, n) : page_items<false>(mover, n);
     const uint32_t blocks = 1 + static_cast<uint32_t>(rng() % 5);
     for (uint32_t b = 0; b < blocks; ++b)
       for (uint32_t item = b; item < items; item += blocks)
         for (uint32_t tid = 0; tid < kPageThreads; ++tid)
-          chunk(item, static_cast<uint32_t>(header[kPageMoves]), tid, [&](uint32_t i) { return moves[i]; });
+          chunk(item, n, tid, [&](uint32_t i) { return moves[i]; }, packed);
   }
 };
 
@@ -487,7 +490,7 @@ void cache_case(uint64_t seed) {
           if (g != ok[0]) die("workgroups disagree");
         for (uint32_t item = 0; ok[0] && item < items; ++item)
           for (uint32_t t = 0; t < static_cast<uint32_t>(kPageThreads); ++t)
-            c.chunk(item, static_cast<uint32_t>(count), t, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; });
+            c.chunk(item, static_cast<uint32_t>(count), t, [&](uint32_t i) { return PageMove{pairs[i], pairs[kFewPairs + i]}; }, false);
       } else if (count) {
         const bool sorted = pick(0, 1);
         launch<K>(1, [&](Lanes<K>& x) { page_copy_plan(x, c.st, c.w, sa.p, sb.p, count, sorted); });
@@ -533,7 +536,8 @@ void corrupt_case(uint64_t seed) {
 
 template <class T>
 double value_of(const char* p) {
-  if constexpr (T::kBytes == 4) return T::get(Mem::loadu<uint32_t>(p));
+  if constexpr (T::kBytes == 1) return 0;
+  else if constexpr (T::kBytes == 4) return T::get(Mem::loadu<uint32_t>(p));
   else return T::get(Mem::loadu<uint16_t>(p));
 }
 
@@ -542,14 +546,14 @@ template <class T, int VEC, bool INTERLEAVED>
 void rotary_case(uint64_t seed, double eps) {
   std::mt19937_64 rng(seed);
   auto pick = [&](int32_t lo, int32_t hi) { return lo + static_cast<int32_t>(rng() % static_cast<uint64_t>(hi - lo + 1)); };
-  const int unit = VEC == 1 ? 1 : 16 / T::kBytes;
-  const int half = (INTERLEAVED && VEC > 1 ? unit / 2 : unit) * pick(1, VEC == 1 ? 9 : 3);
-  const int dim = 2 * half + unit * pick(0, 3);
+  constexpr bool kWide = VEC * T::kBytes == 16, kRaw = T::kBytes == 1;
+  const int half = kRaw ? 0 : (INTERLEAVED ? VEC / 2 : VEC) * pick(1, VEC == 1 ? 9 : 4);
+  const int dim = kWide ? (2 * half + VEC - 1) / VEC * VEC + VEC * pick(kRaw, 3) : 2 * half + pick(kRaw, pick(0, 1) ? 40 : 5);
   const int outer = pick(1, 2), seq = pick(1, 40), heads = pick(1, 11), paged = pick(0, 2);
-  const bool in_place = paged != 1 && pick(0, 2) == 0, turn = !(paged && pick(0, 3) == 0), spread = pick(0, 1);
+  const bool in_place = !kRaw && paged != 1 && pick(0, 2) == 0, turn = !kRaw && !(paged && pick(0, 3) == 0), spread = pick(0, 1);
   const bool heads_minor = paged || pick(0, 1);
   const int tokens = paged ? seq : outer * seq;
-  Exact<uint64_t> freq(half);
+  Exact<uint64_t> freq(std::max(half, 1));
   for (int i = 0; i < half; ++i) freq[i] = static_cast<uint64_t>(std::ldexp(std::pow(100.0, -static_cast<double>(i) / half) / 6.283185307179586, 62)) * 4;
   const int64_t row = static_cast<int64_t>(dim) * T::kBytes;
   RotaryAngles a{};
@@ -563,7 +567,7 @@ void rotary_case(uint64_t seed, double eps) {
   Exact<char> x(static_cast<size_t>(tokens) * heads * row);
   std::normal_distribution<float> normal;
   for (int64_t i = 0; i < static_cast<int64_t>(tokens) * heads * dim; ++i) {
-    const uint32_t v = T::put(normal(rng));
+    const uint32_t v = kRaw ? static_cast<uint32_t>(rng()) : T::put(normal(rng));
     std::memcpy(x.p + i * T::kBytes, &v, T::kBytes);
   }
   j.tokens = tokens, j.seq = seq, j.heads = heads, j.paged = paged;
@@ -632,8 +636,9 @@ void rotary_case(uint64_t seed, double eps) {
   }
   const auto before = x.copy();
   const bool same = buf.dst == x.p;
-  const int rot = turn ? (INTERLEAVED && VEC > 1 ? 2 * half : half) / VEC : 0, rest = turn ? (same ? 0 : (dim - 2 * half) / VEC) : dim / VEC;
-  rotary_shape(&j, rot, rest, j.src_head <= j.src_seq, spread);
+  rotary_units(&j, static_cast<uint32_t>(row), turn ? static_cast<uint32_t>(2 * half * T::kBytes) : 0,
+               static_cast<uint32_t>(VEC * T::kBytes * (INTERLEAVED ? 1 : 2)), T::kBytes, turn && same);
+  rotary_shape(&j, j.src_head <= j.src_seq, spread);
   // in some cases a part of the tile is padding, which stays as it is
   buf.outer = paged ? 1 : pick(1, outer), buf.seq = paged || pick(0, 1) ? seq : pick(1, seq), buf.heads = pick(0, 1) ? heads : pick(1, heads);
   for (uint32_t b = 0; b < j.blocks; ++b)  // its lanes wait for nothing, so that one thread can be all of them in turn
@@ -661,11 +666,11 @@ void rotary_case(uint64_t seed, double eps) {
           if (to[d * T::kBytes] != old) die("a skipped row is written", t, d);
           continue;
         }
-        const double own = value_of<T>(before.data() + at + d * T::kBytes);
         if (!turn || d >= 2 * half) {
           if (std::memcmp(to + d * T::kBytes, before.data() + at + d * T::kBytes, T::kBytes)) die("a value that passes through changed", t, d);
           continue;
         }
+        const double own = value_of<T>(before.data() + at + d * T::kBytes);
         const int i = INTERLEAVED ? d / 2 : d % half;
         const bool second = INTERLEAVED ? d % 2 : d >= half;
         const int other = INTERLEAVED ? d ^ 1 : second ? d - half : d + half;
@@ -706,17 +711,26 @@ int main(int argc, char** argv) {
   for (int i = 0; i < rounds / 4 + 1; ++i) corrupt_case(5000 + i);
   std::printf("corrupt tables: %d\n", rounds / 4 + 1);
   std::fflush(stdout);
+  int shapes = 0;
   for (int i = 0; i < rounds / 4 + 1; ++i) {
-    rotary_case<RotaryF32, 4, false>(10 * i + 1, 1.2e-7);
-    rotary_case<RotaryF32, 4, true>(10 * i + 2, 1.2e-7);
-    rotary_case<RotaryF32, 1, false>(10 * i + 3, 1.2e-7);
-    rotary_case<RotaryF32, 1, true>(10 * i + 4, 1.2e-7);
-    rotary_case<RotaryBF16, 8, false>(10 * i + 5, 0.0078125);
-    rotary_case<RotaryBF16, 8, true>(10 * i + 6, 0.0078125);
-    rotary_case<RotaryBF16, 1, false>(10 * i + 7, 0.0078125);
-    rotary_case<RotaryF16, 8, false>(10 * i + 8, 0.0009765625);
-    rotary_case<RotaryF16, 1, true>(10 * i + 9, 0.0009765625);
+    const auto seed = [&] { return static_cast<uint64_t>(++shapes); };
+    rotary_case<RotaryF32, 4, false>(seed(), 1.2e-7);
+    rotary_case<RotaryF32, 4, true>(seed(), 1.2e-7);
+    rotary_case<RotaryF32, 2, false>(seed(), 1.2e-7);
+    rotary_case<RotaryF32, 2, true>(seed(), 1.2e-7);
+    rotary_case<RotaryF32, 1, false>(seed(), 1.2e-7);
+    rotary_case<RotaryBF16, 8, false>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 8, true>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 4, false>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 4, true>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 2, false>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 2, true>(seed(), 0.0078125);
+    rotary_case<RotaryBF16, 1, false>(seed(), 0.0078125);
+    rotary_case<RotaryF16, 8, false>(seed(), 0.0009765625);
+    rotary_case<RotaryF16, 2, true>(seed(), 0.0009765625);
+    rotary_case<RotaryRaw, 16, false>(seed(), 0);
+    rotary_case<RotaryRaw, 1, false>(seed(), 0);
   }
-  std::printf("rotary: %d shapes\nOK\n", 9 * (rounds / 4 + 1));
+  std::printf("rotary: %d shapes\nOK\n", shapes);
   return 0;
 }
