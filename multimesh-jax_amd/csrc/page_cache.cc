@@ -211,6 +211,14 @@ int vector_bytes(const mmr::RotaryLaunch& l, const std::vector<Row>& rows, int i
   return itemsize;
 }
 
+// Whether every piece of a row that one store instruction writes is whole 128-byte lines.
+bool whole_lines(const mmr::RotaryLaunch& l, const std::vector<Row>& rows, int itemsize) {
+  const int64_t part = static_cast<int64_t>(l.angles.half) * itemsize * (l.interleaved ? 2 : 1);
+  for (const Row& r : rows)
+    if (r.dim * itemsize % 128 || (r.turned && part % 128)) return false;
+  return true;
+}
+
 // Units of the shapes, and the launches.  A call of few rows takes one head a lane, so that its latency is one row's and
 // not four.
 int launch_rows(mmr_context* ctx, mmr::RotaryLaunch* l, const std::vector<Row>& rows, int itemsize) {
@@ -233,7 +241,7 @@ int launch_rows(mmr_context* ctx, mmr::RotaryLaunch* l, const std::vector<Row>& 
     if (mmr::rotary_shape(&j, j.src_head <= j.src_seq, spread) > kMaxRotaryBlocks)
       return fail(MMR_UNSUPPORTED, "a tile of %u tokens of %u heads is more than a launch takes", j.tokens, j.heads);
   }
-  l->past_caches = bytes > kL2Bytes;
+  l->past_caches = bytes > kL2Bytes && whole_lines(*l, rows, itemsize);
   int launches = 0;
   const hipError_t e = mmr::launch_rotary(*l, &launches, mmr::context_stream(ctx));
   mmr::context_count(ctx, launches);

@@ -186,9 +186,10 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState 
   }
 }
 
-// STREAM: a launch that writes more than the caches keep for a reader writes past them (queries, keys and values of 18,001
-// tokens, 443 MB in all: 82.4 -> 79.3 us; the gradient of bf16 [4,32,2048,128] 23.9 -> 20.7 us); what a small one
-// writes, a decode step's queries and keys, stays for the kernel that reads it next.
+// STREAM: a launch that writes more than the caches keep for a reader writes past them, if its stores are whole lines
+// (queries, keys and values of 18,001 tokens, 443 MB in all: 82.4 -> 79.3 us; the gradient of bf16 [4,32,2048,128] 23.9 ->
+// 20.7 us; parts of lines meet in the L2 instead: bf16 rows of 80 with halves of 80 bytes 32.1 us through it, 42.5 past
+// it); what a small one writes, a decode step's queries and keys, stays for the kernel that reads it next.
 template <class T, int VEC, bool INTERLEAVED, bool STREAM, class Args>
 __global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(Args a) {
   Workgroup<kRotaryThreads> x(nullptr);

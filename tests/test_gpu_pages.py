@@ -122,6 +122,7 @@ CACHES = {
     "one token and 12 bytes a page, uneven heads": dict(S=25, Bl=60, P=900, T=1, shape=(1, 3, 2), type="F16", n_dev=2, cut=2),
     "pages over a chunk, heads before tokens": dict(S=12, Bl=9, P=70, T=5, shape=(5, 6, 100), type="F32", n_dev=3, cut=2,
                                                     layout=(3, 1, 2, 0)),
+    "pages of 9 bytes": dict(S=20, Bl=30, P=400, T=3, shape=(3, 3), type="U8", n_pools=1, cut=1),
     "three segments of pages, 8-byte values": dict(S=300, Bl=50, P=9001, T=2, shape=(2, 1), type="F64", n_pools=1, cut=1),
 }
 
@@ -308,6 +309,14 @@ ROTARY = [
     ((6, 3, 600), 0, 0, 2, None, 600, False, "F32", {}, 1.0, 0),
     ((6, 3, 1100), 0, 0, 1, None, 1100, False, "F32", dict(frequencies=True), 1.0, 9),
     ((7, 2, 2), 0, 0, 1, None, 2, False, "BF16", {}, 1.0, 0),
+    # turned parts of 8, 4 and 2 bytes' multiples, rests of many and of few bytes
+    ((9, 3, 40), 0, 0, 2, None, 40, False, "BF16", {}, 1.0, 0),
+    ((9, 3, 45), 0, 1, 2, None, 12, False, "BF16", {}, 1.0, 100),
+    ((9, 3, 21), 0, 0, 1, None, 20, True, "F16", {}, 1.0, 0),
+    ((9, 3, 31), 0, 0, 1, None, 6, True, "F32", {}, 1.0, 0),
+    ((9, 3, 31), 0, 0, 1, None, 28, False, "F32", {}, 1.0, 0),
+    ((9, 3, 16), 0, 0, 1, None, 14, True, "BF16", {}, 1.0, 50),
+    ((9, 3, 35), 0, 0, 1, None, 6, False, "F16", {}, 1.0, 50),
     ((40, 3, 16), 0, 0, 20, None, 16, False, "BF16", {}, 1.0, 0),   # 20 buffers: more than one launch takes
     ((1, 1, 8), 0, 0, 1, None, 8, True, "F16", {}, 1.0, 12345),
     ((300, 9, 32, 128), 1, 1, 3, None, 128, False, "BF16", {}, 1.0, 7),  # 22 MB
