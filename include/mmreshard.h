@@ -535,8 +535,12 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
  * so on.  extend, fork and copy check all their entries first and change nothing at all if one is bad; the reason is
  * kept until mmr_pages_status reads it.  Pages are given out lowest free id first, in the order of the entries.
+ * MMR_PAGES_NONE in place of a sequence (fork: of the child; copy: of the destination) is no entry and is passed over, so
+ * that a graph captured for the largest batch can be replayed for smaller ones.
  * ------------------------------------------------------------------------- */
 typedef struct mmr_pages mmr_pages;
+
+#define MMR_PAGES_NONE (-1)
 
 #define MMR_PAGES_BAD_SEQUENCE 1u   /* a sequence outside [0, S) */
 #define MMR_PAGES_BAD_PAGE 2u       /* a page outside the pools, in an argument or in a row of the table */
@@ -609,7 +613,8 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
 
 /* New tokens into the pages of a cache, after mmr_pages_extend made room for them: tokens begins[i] .. begins[i + 1] - 1
  * of k (and v, q) are the last ones of sequences[i], so the first stands at position lengths - (begins[i + 1] -
- * begins[i]).  begins: n + 1 ascending values; tokens before the first and after the last are padding and left out.  k
+ * begins[i]).  begins: n + 1 ascending values; tokens before the first and after the last are padding and left out, as
+ * are those of a sequence MMR_PAGES_NONE; the sequences are distinct (of two entries of one, either may be kept).  k
  * goes to pool k_pool, v (or NULL) to pool v_pool: stores [tokens, heads, dim], heads sharded as in the pool.  With a
  * rotary plan k is turned on its way, and q (any heads, [tokens, heads, dim], or NULL) is turned into q_out (or in
  * place).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.  Tokens of an entry whose

@@ -16,6 +16,7 @@ MMR_PLAN_ALL_GENERIC, MMR_PLAN_NO_AUTOTUNE, MMR_PLAN_NO_SPAN = 1, 2, 4
 MMR_PLAN_NO_INLINE, MMR_PLAN_NO_SEGMENT_TABLES = 8, 16
 MMR_CHECK_INVARIANTS = 1
 MMR_STATIC_SCRATCH_BYTES = 1 << 20
+MMR_PAGES_NONE = -1
 PAGES_FLAGS = {"BAD_SEQUENCE": 1, "BAD_PAGE": 2, "OUT_OF_PAGES": 4, "TOO_LONG": 8, "REPEATED": 16, "NOT_EMPTY": 32,
                "SHARED_TAIL": 64, "OVERLAP": 128, "BAD_COUNT": 256}
 ROTARY_SCALINGS = {None: 0, "linear": 1, "parts": 2}

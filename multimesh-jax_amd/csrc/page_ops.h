@@ -192,6 +192,7 @@ MMR_HD uint32_t page_fork_entry(X& x, const PageState& st, const PageWork& w, in
                                 int32_t* src) {
   *len = 0;
   *src = -1;
+  if (child == MMR_PAGES_NONE) return 0;
   if (parent < 0 || parent >= st.S || child < 0 || child >= st.S) return MMR_PAGES_BAD_SEQUENCE;
   uint32_t flags = 0;
   const int32_t l = st.lengths[parent];
@@ -244,6 +245,7 @@ MMR_HD void page_fork_rows(X& x, const PageState& st, const PageWork& w, const i
   uint32_t bad = 0;
   for (int32_t e = static_cast<int32_t>(block); e < n; e += static_cast<int32_t>(blocks)) {
     const int32_t len = w.len[e], rank = w.rank[e], child = children[e];
+    if (child == MMR_PAGES_NONE) continue;
     const int32_t full = static_cast<int32_t>(fdiv(static_cast<uint32_t>(len), st.div_T));
     const int32_t* from = st.table + static_cast<int64_t>(parents[e]) * st.B;
     int32_t* to = st.table + static_cast<int64_t>(child) * st.B;
@@ -279,7 +281,9 @@ MMR_HD void page_extend_plan(X& x, const PageState& st, const PageWork& w, int32
     int32_t need = 0, old = 0;
     if (e < n) {
       const int32_t s = slots[e], c = counts[e];
-      if (s < 0 || s >= st.S) {
+      if (s == MMR_PAGES_NONE) {
+        // no entry
+      } else if (s < 0 || s >= st.S) {
         bad |= MMR_PAGES_BAD_SEQUENCE;
       } else {
         if (x.atomic_exch(&w.mark[s], 1)) bad |= MMR_PAGES_REPEATED;
@@ -323,7 +327,8 @@ MMR_HD void page_extend_plan(X& x, const PageState& st, const PageWork& w, int32
       st.table[static_cast<int64_t>(slots[lo]) * st.B + page_blocks(st, w.len[lo]) + (k - w.rank[lo])] = page;
       st.refs[page] = 1;
     }
-    for (int32_t e = x.tid; e < n; e += X::kThreads) st.lengths[slots[e]] = w.len[e] + counts[e];
+    for (int32_t e = x.tid; e < n; e += X::kThreads)
+      if (slots[e] != MMR_PAGES_NONE) st.lengths[slots[e]] = w.len[e] + counts[e];
   }
   if (rows) pages.publish(x);
   if (x.tid == 0) {
@@ -339,6 +344,7 @@ MMR_HD void page_extend_rows(X& x, const PageState& st, const PageWork& w, int32
   if (!w.header[kPageRows]) return;
   const FreePages<X, kSegment> pages(x, w, shared, true);
   for (int32_t e = static_cast<int32_t>(x.block); e < n; e += static_cast<int32_t>(x.blocks)) {
+    if (slots[e] == MMR_PAGES_NONE) continue;
     const int32_t old = w.len[e], all = old + counts[e], rank = w.rank[e], have = page_blocks(st, old);
     int32_t* row = st.table + static_cast<int64_t>(slots[e]) * st.B + have;
     for (int32_t i = x.tid, need = page_blocks(st, all) - have; i < need; i += X::kThreads) {
@@ -357,7 +363,7 @@ MMR_HD void page_free(X& x, const PageState& st, const PageWork& w, int32_t* sha
   const int32_t s = slots[x.block];
   uint32_t bad = 0;
   if (s < 0 || s >= st.S) {  // uniform over the workgroup
-    if (x.tid == 0) x.atomic_or(&w.header[kPageStatus], MMR_PAGES_BAD_SEQUENCE);
+    if (x.tid == 0 && s != MMR_PAGES_NONE) x.atomic_or(&w.header[kPageStatus], MMR_PAGES_BAD_SEQUENCE);
     return;
   }
   if (x.tid == 0) shared[0] = x.atomic_exch(&st.lengths[s], 0);
@@ -454,6 +460,7 @@ MMR_HD void page_copy_plan(X& x, const PageState& st, const PageWork& w, const i
   uint32_t bad = 0;
   for (int32_t e = x.tid; e < n; e += X::kThreads) {
     const int32_t s = src[e], d = dst[e];
+    if (d == MMR_PAGES_NONE) continue;
     if (s < 0 || s >= st.P || d < 0 || d >= st.P) bad |= MMR_PAGES_BAD_PAGE;
     else if (s != d && x.atomic_exch(&w.mark[d], e + 1)) bad |= MMR_PAGES_REPEATED;
   }
@@ -501,12 +508,13 @@ MMR_HD bool page_copy_few(X& x, const PageState& st, const PageWork& w, int32_t*
   int32_t s = -1, d = -1;
   if (x.tid < n) {
     s = src[x.tid], d = dst[x.tid];
+    if (d == MMR_PAGES_NONE) s = d;  // no pair, and no move, as for a page copied onto itself
     shared[x.tid] = s;
     shared[kFewPairs + x.tid] = d;
   }
   x.sync();
   uint32_t bad = 0;
-  if (x.tid < n) {
+  if (x.tid < n && d != MMR_PAGES_NONE) {
     if (s < 0 || s >= st.P || d < 0 || d >= st.P) {
       bad |= MMR_PAGES_BAD_PAGE;
     } else if (s != d) {

@@ -199,7 +199,7 @@ MMR_HD bool rotary_place(X& x, const RotaryPages& pg, int32_t wave_token, int32_
   const int32_t begin = pg.begins[entry], end = pg.begins[entry + 1], slot = pg.slots[entry];
   if (t < begin) return false;  // before the first one
   if (slot < 0 || slot >= pg.S) {
-    *bad = MMR_PAGES_BAD_SEQUENCE;
+    *bad = slot == MMR_PAGES_NONE ? 0 : MMR_PAGES_BAD_SEQUENCE;
     return false;
   }
   const int64_t p = static_cast<int64_t>(pg.lengths[slot]) - end + t;

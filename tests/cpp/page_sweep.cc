@@ -241,6 +241,7 @@ uint32_t model_extend(const Cache& c, Model* m, const std::vector<int32_t>& s, c
   std::set<int32_t> seen;
   int64_t need = 0;
   for (size_t e = 0; e < s.size(); ++e) {
+    if (s[e] == MMR_PAGES_NONE) continue;
     if (s[e] < 0 || s[e] >= c.S) {
       bad |= MMR_PAGES_BAD_SEQUENCE;
       continue;
@@ -263,6 +264,7 @@ uint32_t model_extend(const Cache& c, Model* m, const std::vector<int32_t>& s, c
   if (bad) return bad;
   size_t k = 0;
   for (size_t e = 0; e < s.size(); ++e) {
+    if (s[e] == MMR_PAGES_NONE) continue;
     const int32_t old = m->lengths[s[e]];
     for (int32_t b = blocks_of(old, c.T); b < blocks_of(old + n[e], c.T); ++b) {
       m->table[static_cast<size_t>(s[e]) * c.B + b] = f[k];
@@ -279,6 +281,7 @@ uint32_t model_fork(const Cache& c, Model* m, const std::vector<int32_t>& p, con
   size_t need = 0;
   const std::vector<int32_t> lengths = m->lengths;
   for (size_t e = 0; e < p.size(); ++e) {
+    if (ch[e] == MMR_PAGES_NONE) continue;
     if (p[e] < 0 || p[e] >= c.S || ch[e] < 0 || ch[e] >= c.S) {
       bad |= MMR_PAGES_BAD_SEQUENCE;
       continue;
@@ -300,6 +303,7 @@ uint32_t model_fork(const Cache& c, Model* m, const std::vector<int32_t>& p, con
   if (bad) return bad;
   size_t k = 0;
   for (size_t e = 0; e < p.size(); ++e) {
+    if (ch[e] == MMR_PAGES_NONE) continue;
     const int32_t l = lengths[p[e]], full = l / c.T;
     const size_t from = static_cast<size_t>(p[e]) * c.B, to = static_cast<size_t>(ch[e]) * c.B;
     for (int32_t i = 0; i < full; ++i) {
@@ -319,6 +323,7 @@ uint32_t model_fork(const Cache& c, Model* m, const std::vector<int32_t>& p, con
 uint32_t model_free(const Cache& c, Model* m, const std::vector<int32_t>& s) {
   uint32_t bad = 0;
   for (int32_t q : s) {
+    if (q == MMR_PAGES_NONE) continue;
     if (q < 0 || q >= c.S) {
       bad |= MMR_PAGES_BAD_SEQUENCE;
       continue;
@@ -354,6 +359,7 @@ uint32_t model_copy(const Cache& c, Model* m, const std::vector<int32_t>& s, con
   uint32_t bad = 0;
   std::set<int32_t> dsts;
   for (size_t e = 0; e < s.size(); ++e) {
+    if (d[e] == MMR_PAGES_NONE) continue;
     if (s[e] < 0 || s[e] >= c.P || d[e] < 0 || d[e] >= c.P) bad |= MMR_PAGES_BAD_PAGE;
     else if (s[e] != d[e] && !dsts.insert(d[e]).second) bad |= MMR_PAGES_REPEATED;
   }
@@ -362,7 +368,8 @@ uint32_t model_copy(const Cache& c, Model* m, const std::vector<int32_t>& s, con
   if (bad) return bad;
   for (auto& pool : m->pools) {
     const auto before = pool;
-    for (size_t e = 0; e < s.size(); ++e) pool[d[e]] = before[s[e]];
+    for (size_t e = 0; e < s.size(); ++e)
+      if (d[e] != MMR_PAGES_NONE) pool[d[e]] = before[s[e]];
   }
   return 0;
 }
@@ -396,7 +403,7 @@ void cache_case(uint64_t seed) {
     if (op == 0 || op == 1) {
       int n = pick(0, S);
       for (int e = 0; e < n; ++e) {
-        a.push_back(wild ? pick(-1, S) : seqs[e]);
+        a.push_back(wild ? pick(-2, S) : pick(0, 9) ? seqs[e] : MMR_PAGES_NONE);
         const int32_t room = c.st.capacity - std::min(c.st.capacity, c.lengths[seqs[e]]);
         b.push_back(wild ? pick(-1, 2 * T) : pick(0, std::max(0, room) ? std::min(room, pick(0, 2) ? 2 * T : B * T) : 0));
       }
@@ -421,7 +428,7 @@ void cache_case(uint64_t seed) {
       const int n = wild ? pick(0, S) : pick(0, static_cast<int32_t>(empty.size()));
       for (int e = 0; e < n; ++e) {
         a.push_back(pick(wild ? -1 : 0, wild ? S : S - 1));
-        b.push_back(wild ? pick(-1, S) : empty[e]);
+        b.push_back(wild ? pick(-2, S) : pick(0, 9) ? empty[e] : MMR_PAGES_NONE);
       }
       const uint32_t want = model_fork(c, &m, a, b);
       Exact<int32_t> sa(a.size()), sb(b.size());
@@ -442,7 +449,7 @@ void cache_case(uint64_t seed) {
       c.check(m, "fork");
     } else if (op == 3) {
       const int n = pick(0, S);
-      for (int e = 0; e < n; ++e) a.push_back(wild ? pick(-1, S) : seqs[pick(0, S - 1)]);
+      for (int e = 0; e < n; ++e) a.push_back(wild ? pick(-2, S) : pick(-1, 0) ? MMR_PAGES_NONE : seqs[pick(0, S - 1)]);
       const uint32_t want = model_free(c, &m, a);
       Exact<int32_t> sa(a.size());
       std::copy(a.begin(), a.end(), sa.p);
@@ -471,7 +478,7 @@ void cache_case(uint64_t seed) {
       const int32_t cut = pick(0, P);  // sources from one side, destinations from the other
       for (int e = 0; e < n && (wild || (cut > 0 && cut + e < P)); ++e) {
         a.push_back(wild ? pick(-1, P) : pick(0, 9) == 0 ? ids[cut + e] : ids[pick(0, cut - 1)]);
-        b.push_back(wild ? pick(0, P) : ids[cut + e]);
+        b.push_back(wild ? pick(-2, P) : pick(0, 9) ? ids[cut + e] : MMR_PAGES_NONE);
       }
       const uint32_t want = model_copy(c, &m, a, b);
       const int32_t count = static_cast<int32_t>(a.size());
@@ -594,7 +601,7 @@ void rotary_case(uint64_t seed, double eps) {
     std::sort(cuts.begin(), cuts.end());
     for (int e = 0; e <= n; ++e) begins[e] = cuts[e];
     for (int e = 0; e < n; ++e) {
-      slots[e] = pick(0, 12) == 0 ? (pick(0, 1) ? -1 : S) : order[e];
+      slots[e] = pick(0, 12) == 0 ? (pick(0, 1) ? -2 : S) : pick(0, 12) == 0 ? MMR_PAGES_NONE : order[e];
       const int32_t count = begins[e + 1] - begins[e];
       if (slots[e] >= 0 && slots[e] < S) {
         lengths[slots[e]] = count + pick(0, 9);
@@ -602,7 +609,7 @@ void rotary_case(uint64_t seed, double eps) {
       }
       for (int32_t t = begins[e]; t < begins[e + 1]; ++t) {
         if (slots[e] < 0 || slots[e] >= S) {
-          want_status |= MMR_PAGES_BAD_SEQUENCE;
+          if (slots[e] != MMR_PAGES_NONE) want_status |= MMR_PAGES_BAD_SEQUENCE;
           continue;
         }
         const int32_t p = lengths[slots[e]] - count + (t - begins[e]);

@@ -203,7 +203,7 @@ def test_rows_longer_than_a_workgroup(ctx):
 
 BAD = [
     ("extend", ([0, 99], [1, 1]), {"BAD_SEQUENCE"}),
-    ("extend", ([0, -1], [1, 1]), {"BAD_SEQUENCE"}),
+    ("extend", ([0, -2], [1, 1]), {"BAD_SEQUENCE"}),
     ("extend", ([3, 4, 3], [1, 1, 1]), {"REPEATED"}),
     ("extend", ([3], [-1]), {"TOO_LONG"}),
     ("extend", ([3], [33]), {"TOO_LONG"}),
@@ -218,7 +218,8 @@ BAD = [
     ("copy", ([0, 20], [20, 21]), {"OVERLAP"}),
     ("copy", ([0, 1], [1, 0]), {"OVERLAP"}),
     ("copy", ([0, 24], [20, 21]), {"BAD_PAGE"}),
-    ("copy", ([0, 1], [-1, 21]), {"BAD_PAGE"}),
+    ("copy", ([0, 1], [-2, 21]), {"BAD_PAGE"}),
+    ("copy", ([0, -1], [22, 21]), {"BAD_PAGE"}),
 ]
 
 
@@ -240,11 +241,65 @@ def test_a_call_with_a_bad_entry_changes_nothing(ctx, name, args, flags):
 def test_free_takes_a_sequence_once_and_skips_bad_entries(ctx):
     p = Pair(ctx, S=8, Bl=8, P=24, T=4, shape=(4, 2, 8), type="BF16", seed=9)
     p.op("extend", [0, 1, 2], [13, 20, 4])
-    p.cache.Free(p.ids([1, 99, 1, 5, -1, 1]))
+    p.cache.Free(p.ids([1, 99, 1, 5, -2, 1]))
     p.model.free([1])
     got, used = p.cache.Status()
     assert got == ["BAD_SEQUENCE"] and used == 5
     p.check()
+    p.close()
+
+
+def test_entries_that_are_none_are_passed_over(ctx):
+    """A batch smaller than the arrays: MMR_PAGES_NONE stands where there is no entry, whatever stands beside it."""
+    none = B.MMR_PAGES_NONE
+    p = Pair(ctx, S=8, Bl=8, P=40, T=4, shape=(4, 2, 8), type="BF16", seed=9)
+    p.cache.Extend(p.ids([none, 0, none, 1, 2, none]), p.ids([99999, 13, -7, 20, 4, 1]))
+    p.model.extend([0, 1, 2], [13, 20, 4])
+    p.check()
+    p.cache.Fork(p.ids([99, 0, -4]), p.ids([none, 3, none]))
+    p.model.fork([0], [3])
+    p.check()
+    p.cache.Copy(p.ids([0, 1, -9]), p.ids([30, none, none]))
+    p.model.copy([0], [30])
+    p.cache.Copy(p.ids([0, -9] * 18 + [2]), p.ids([none, none] * 18 + [31]))
+    p.model.copy([2], [31])
+    p.cache.Free(p.ids([none, 2, none]))
+    p.model.free([2])
+    p.check()
+    k = values(np.random.Generator(np.random.PCG64(1)), (5, 2, 8), "BF16")
+    p.cache.Write(p.ids([none, 1, none]), p.ids([0, 2, 3, 5]), 0, split(ctx, k, "BF16", 1, 1))
+    p.model.pools[0][p.model.table[1, 4], 3] = k[2]
+    p.check()
+    for call in (p.cache.Extend, p.cache.Fork, p.cache.Copy):
+        call(p.ids([0, 1]), p.ids([none, none])) if call != p.cache.Extend else call(p.ids([none, none]), p.ids([0, 1]))
+    p.check()
+    p.close()
+
+
+def test_calls_from_two_threads(ctx):
+    """Two threads on one cache: every call is whole, whichever comes first."""
+    import threading
+    p = Pair(ctx, S=64, Bl=8, P=400, T=4, shape=(4, 8), type="BF16", n_pools=1, seed=9)
+    ids = [[p.ids([s, s + 1]) for s in range(t * 32, t * 32 + 32, 2)] for t in range(2)]
+    counts = p.ids([6, 9])
+
+    def work(t):
+        for a in ids[t]:
+            p.cache.Extend(a, counts)
+        for a in ids[t][::2]:
+            p.cache.Free(a)
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    table, lengths, refs = p.tables()
+    want = np.array([0 if s // 2 % 2 == 0 else (6, 9)[s % 2] for s in range(64)])
+    assert np.array_equal(lengths, want)
+    held = np.concatenate([table[s, :p.model.blocks(n)] for s, n in enumerate(want)])
+    assert len(set(held)) == len(held) and refs.sum() == len(held) and (refs[held] == 1).all()
+    assert p.cache.Status() == ([], len(held))
     p.close()
 
 
