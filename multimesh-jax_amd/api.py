@@ -342,7 +342,7 @@ def _ids(ctx: "ReshardContext", a, what: str) -> Tuple[int, int]:
     """(device address, entries) of an int32 array in the memory of the context's GPU: a StoreHandle (S32, one device,
     rank 1), an array object of a GPU framework (int32, contiguous), or such a pair itself."""
     if hasattr(a, "data_ptr"):
-        if not getattr(a, "is_cuda", False) or a.get_device() != ctx.hip_device:
+        if a.get_device() != ctx.hip_device:  # -1: host memory
             raise ValueError("%s: the array is not in the memory of GPU %d" % (what, ctx.hip_device))
         if not _is_int32(a.dtype) or not a.is_contiguous():
             raise ValueError("%s: ids are int32 and contiguous, not %s" % (what, a.dtype))

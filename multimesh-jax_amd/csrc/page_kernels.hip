@@ -8,7 +8,7 @@
 namespace mmr {
 namespace {
 
-typedef DeviceMem<true, true> StreamMem;  // every byte is touched once
+typedef RowMem<true, true> StreamMem;  // every byte is touched once
 
 // A workgroup of K threads.
 template <int K>
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kPageThreads) void mmr_page_apply_kernel(PageState 
   const uint32_t step = gridDim.x - row_blocks;
   for (uint32_t at = blockIdx.x - row_blocks; at < (items + 511u) / 512u * 512u; at += step) {
     const uint32_t item = chunk_index(at, 64);  // runs of 64 neighbours share an XCD
-    typedef DeviceMem<KIND != 1, true> M;
+    typedef RowMem<KIND != 1, true> M;
     if (item < items) page_move_chunk<M, ALIGNED, PACKED>(mv, [&](uint32_t i) { return w.moves[i]; }, moves, item, threadIdx.x);
   }
 }
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kRotaryThreads) void mmr_rotary_kernel(Args a) {
   const RotaryBuffer& b = a.buffers[blockIdx.y];
   const RotaryShape& j = a.shapes[Args::kShapes == 1 ? 0 : b.shape];
   if (x.block >= j.blocks) return;  // uniform over the workgroup
-  rotary_block<DeviceMem<false, STREAM>, T, VEC, INTERLEAVED>(x, a.angles, a.pages, j, b);
+  rotary_block<RowMem<false, STREAM>, T, VEC, INTERLEAVED>(x, a.angles, a.pages, j, b);
 }
 
 template <class Args>
