@@ -274,9 +274,10 @@ constexpr uint64_t kMaxMoveBlocks = 1u << 18;
 // Up to so many pages the plan of a compact lists the moves itself, in at most 8 rounds (compact of 16,384 pages of 256
 // bytes: 19.9 us, with a launch for the list 21.8; of 32,768: 30.1 and 23.7).
 constexpr int32_t kCompactWhole = 16384;
-// Up to so many chunks a copy of few pairs is one launch, whose workgroups each check all pairs (64 chunks: 4.6 us, in
-// two launches 6.9; 1,024 chunks of 64 pairs: 9.5 and 8.1; 4,096: 23.3 and 17.2).
-constexpr uint64_t kFewChunks = 256;
+// A copy of few pairs is one launch, whose workgroups (one a chunk) each check all pairs, up to so many workgroups times
+// pairs: 4 pairs of 1,024 chunks 4.6 us, in two launches 7.7; 16 of 1,024 5.5 and 7.5; 32 of 512 5.9 and 7.9; 32 of 2,048
+// 9.8 and 13.1; but 64 of 1,024 9.7 and 8.8, 32 of 8,192 32.5 and 29.2.
+constexpr uint64_t kFewChecks = 48 * 1024;
 
 template <int KIND>
 hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLaunch& mv, const int32_t* parents,
@@ -344,7 +345,7 @@ hipError_t launch_page_compact(const PageState& st, const PageWork& w, const Pag
 hipError_t launch_page_copy(const PageState& st, const PageWork& w, const int32_t* src, const int32_t* dst, int32_t n,
                             const PageMoveLaunch& mv, hipStream_t stream, int* launches) {
   const uint64_t items = static_cast<uint64_t>(n) * mv.mover.n_buffers * mv.mover.chunks;
-  if (n <= kFewPairs && items <= kFewChunks) {
+  if (n <= kFewPairs && items * static_cast<uint64_t>(n) <= kFewChecks) {
     const dim3 grid(static_cast<uint32_t>(items));
     if (mv.aligned) hipLaunchKernelGGL(mmr_page_copy_few_kernel<true>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
     else hipLaunchKernelGGL(mmr_page_copy_few_kernel<false>, grid, dim3(kPageThreads), 0, stream, st, w, mv.mover, src, dst, n);
