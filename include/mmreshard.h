@@ -526,7 +526,8 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  * page alive that no sequence uses (refs + 1).
  *
  * Arrays of sequences, pages and counts are int32 in device memory, 4-byte aligned, read when the call's kernels run:
- * the caller orders their writes before the call on the context's stream.  Every call is asynchronous, allocates
+ * the caller orders their writes before the call on the context's stream, and keeps them until the stream has passed it
+ * (arrays of a GPU framework that works on another stream: let its allocator know, or wait).  Every call is asynchronous, allocates
  * nothing, copies nothing from the host and may be captured into a HIP graph; calls of one cache are ordered by the
  * context's stream, and graphs captured from one cache must not run at the same time, as they share its tables and
  * workspace.  (The first call after a pool was offloaded and reloaded enters its buffers anew and is refused while

@@ -372,8 +372,9 @@ class RotaryPlan:
 
 class PageCache:
     """Pages of keys and values in a set of stores (include/mmreshard.h, "Page cache"); made by
-    ReshardContext.CreatePages.  Sequences, pages and counts are int32 arrays in device memory (see _ids).  Calls are
-    asynchronous; what an entry had wrong is told by Status."""
+    ReshardContext.CreatePages.  Sequences, pages and counts are int32 arrays in device memory (see _ids), which the
+    caller keeps until the context's stream has passed the call; B.MMR_PAGES_NONE is no entry.  Calls are asynchronous;
+    what an entry had wrong is told by Status."""
 
     def __init__(self, ctx: "ReshardContext", handle: C.c_void_p):
         self._ctx, self._h, self._lib = ctx, handle, ctx._lib

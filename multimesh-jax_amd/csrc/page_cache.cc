@@ -307,7 +307,8 @@ int mmr_pages_create(mmr_context* ctx, mmr_store* const* pools, int32_t n_pools,
     return here;
   };
   const size_t header = take(mmr::kPageHeaderInts, 4), mark = take(std::max(S, P), 4), cleared = at;
-  const size_t seg_free = take(segments, 4), seg_before = take(segments, 4), free_ids = take(ids, 4), live_ids = take(ids, 4), len = take(S, 4), rank = take(S, 4);
+  const size_t seg_free = take(segments, 4), seg_before = take(segments, 4), free_ids = take(ids, 4), live_ids = take(ids, 4);
+  const size_t len = take(S, 4), rank = take(S, 4);
   const size_t moves = take(std::max(S, P), sizeof(mmr::PageMove)), map = take(P, 4);
   p->buffers_at = take(buffers, sizeof(mmr::PageBuffer));
   p->owner = ctx;

@@ -46,6 +46,7 @@ struct RotaryShape {
   uint16_t head_lanes;                   // rows of a workgroup along the heads ...
   uint16_t token_lanes;                  // ... and along the tokens
   uint16_t head_steps;                   // heads a lane takes, head_lanes apart
+  uint32_t rest_two;                     // a unit of the rest is two vectors, like those of the rotated part
   uint32_t paged;                        // 1: into pages; 2: by the positions of a paged write, beside the source
   FastDiv div_seq, div_head_groups;
 };
@@ -216,7 +217,8 @@ MMR_HD bool rotary_place(X& x, const RotaryPages& pg, int32_t wave_token, int32_
 }
 
 // Lane (row, unit) of workgroup `block` of a buffer.  A unit is what a lane turns: the two vectors that hold VEC pairs, or,
-// interleaved, one vector of VEC / 2 pairs; in the rest of the row it is 16 bytes, the last ones slid back to end with the
+// interleaved, one vector of VEC / 2 pairs; in the rest of the row it is two vectors as well, where they are whole ones of
+// 16 bytes (half of bf16 rows of 128 turned: 37.0 -> 34.4 us for 12,000 tokens of 32 heads), and otherwise 16 bytes, the last ones slid back to end with the
 // row (they repeat their neighbour's bytes, with the same values), or one element if the rest is shorter.  The rows are
 // loaded before the position is looked up: the look-up is a chain of four loads.
 template <class M, class T, int VEC, bool INTERLEAVED, class X>
@@ -243,6 +245,11 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
       *off_b = *off_a + static_cast<int64_t>(a.half) * T::kBytes;
     } else {
       const uint32_t at = unit - j.rot_units;
+      if (kTwo && kWide && j.rest_two) {
+        *off_a = static_cast<int64_t>(j.rest_at) + at * 16;
+        *off_b = *off_a + j.rest_bytes / 2;
+        return;
+      }
       uint32_t in_rest = at * T::kBytes;
       if (j.rest_bytes >= 16) in_rest = at * 16 + 16 <= j.rest_bytes ? at * 16 : j.rest_bytes - 16;
       *off_a = *off_b = static_cast<int64_t>(j.rest_at) + in_rest;
@@ -263,7 +270,7 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
         else if (T::kBytes == 4) rest[k].x = M::template loadu<uint32_t>(from);
         else if (T::kBytes == 2) rest[k].x = M::template loadu<uint16_t>(from);
         else rest[k].x = M::template loadu<uint8_t>(from);
-        if (kTwo && unit < j.rot_units) vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
+        if (kTwo && (unit < j.rot_units || (kWide && j.rest_two))) vb[k].template load<M>(M::cplace(src + (h * j.src_head + off_b)));
       }
     }
   };
@@ -348,7 +355,10 @@ MMR_HD void rotary_block(X& x, const RotaryAngles& a, const RotaryPages& pages, 
         const uint32_t h = h0 + k * j.head_lanes;
         if (k >= j.head_steps || h >= b.heads) continue;
         const typename M::ptr to = M::place(dst + (h * j.dst_head + off_a));
-        if (kWide) va[k].template store<M>(to);
+        if (kWide) {
+          va[k].template store<M>(to);
+          if (kTwo && j.rest_two) vb[k].template store<M>(M::place(dst + (h * j.dst_head + off_b)));
+        }
         else if (j.rest_bytes >= 16) M::template storeu<V16>(to, rest[k]);
         else if (T::kBytes == 4) M::template storeu<uint32_t>(to, rest[k].x);
         else if (T::kBytes == 2) M::template storeu<uint16_t>(to, static_cast<uint16_t>(rest[k].x));
@@ -367,7 +377,8 @@ inline void rotary_units(RotaryShape* j, uint32_t bytes, uint32_t turned, uint32
   j->rot_units = turned / unit_bytes;
   j->rest_at = turned;
   j->rest_bytes = in_place ? 0 : bytes - turned;  // in place, what is not turned stays
-  j->units = j->rot_units + (j->rest_bytes >= 16 ? (j->rest_bytes + 15) / 16 : j->rest_bytes / element);
+  j->rest_two = element > 1 && unit_bytes == 32 && j->rest_bytes > 0 && j->rest_bytes % 32 == 0;
+  j->units = j->rot_units + (j->rest_two ? j->rest_bytes / 32 : j->rest_bytes >= 16 ? (j->rest_bytes + 15) / 16 : j->rest_bytes / element);
 }
 
 // How the rows of a shape are dealt to workgroups; returns how many that takes.  `spread`: one head a lane, for launches
