@@ -13,7 +13,7 @@
 // free ids, in order, and their count; the plan, one workgroup, sums the counts and looks the k-th free page up by a
 // binary search over them.  A pool of few segments is scanned by the plan itself.  (All in one launch, the plan being
 // the part of the workgroup that arrives last, needs fences between the XCDs' caches, which cost more than a launch:
-// extend over 98 segments 50 us, over two 16 us and up to 54 us behind large copies, where one segment takes 6.)
+// extend over 98 segments 50 us, over two 16, where one segment takes 6.)
 //
 // X is the workgroup: the GPU's (page_kernels.hip) or, in the tests, a set of host threads.  It has kThreads, tid,
 // block, blocks, sync(), scan(v, &total) (exclusive sum over the threads), any(flags) (bitwise or over the threads),
