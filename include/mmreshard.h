@@ -534,7 +534,8 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  * capturing, and a graph captured before that, or from a handle that was destroyed since, must not be replayed.)
  *
  * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
- * so on.  extend, fork and copy check all their entries first and change nothing at all if one is bad; the reason is
+ * so on.  extend, fork and copy check all their entries first, fork the pages that are to be shared or copied too, and
+ * change nothing at all if one is bad; the reason is
  * kept until mmr_pages_status reads it.  Pages are given out lowest free id first, in the order of the entries.
  * MMR_PAGES_NONE in place of a sequence (fork: of the child; copy: of the destination) is no entry and is passed over, so
  * that a graph captured for the largest batch can be replayed for smaller ones.
@@ -551,7 +552,7 @@ typedef struct mmr_pages mmr_pages;
 #define MMR_PAGES_NOT_EMPTY 32u     /* fork into a sequence that holds tokens */
 #define MMR_PAGES_SHARED_TAIL 64u   /* extend of a sequence whose last, partly filled page has other users */
 #define MMR_PAGES_OVERLAP 128u      /* copy: a destination is also the source of another pair */
-#define MMR_PAGES_BAD_COUNT 256u    /* free, compact: refs out of step with the table (a page in a row that nobody uses) */
+#define MMR_PAGES_BAD_COUNT 256u    /* fork, free, compact: refs out of step with the table (a page in a row that nobody uses) */
 
 /* page_tokens: tokens a page holds.  At most 2^21 sequences and 2^24 pages.  The handle lives until mmr_pages_destroy or
  * the end of the context; its stores must outlive it. */

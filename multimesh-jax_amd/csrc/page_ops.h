@@ -41,7 +41,16 @@ struct PageState {
   FastDiv div_T;
 };
 
-enum PageHeader { kPageOk = 1, kPageMoves = 2, kPageStatus = 3, kPageLive = 4, kPageFree = 5, kPageRows = 6, kPageHeaderInts = 64 };
+enum PageHeader {
+  kPageOk = 1,
+  kPageMoves = 2,
+  kPageStatus = 3,
+  kPageLive = 4,
+  kPageFree = 5,
+  kPageRows = 6,
+  kPageForkBad = 7,  // what page_fork_check found; zero between calls
+  kPageHeaderInts = 64
+};
 
 struct PageWork {
   int32_t* header;
@@ -186,6 +195,32 @@ MMR_HD void page_verdict(X& x, const PageWork& w, uint32_t bad, int32_t moves, i
   if (bad) x.atomic_or(&w.header[kPageStatus], static_cast<int32_t>(bad));
 }
 
+// A page that a sequence with tokens names: it is there, and somebody uses it.
+MMR_HD uint32_t page_held(const PageState& st, int32_t page) {
+  if (page < 0 || page >= st.P) return MMR_PAGES_BAD_PAGE;
+  return st.refs[page] > 0 ? 0 : MMR_PAGES_BAD_COUNT;
+}
+
+// Full pages of entry e's parent; 0 where page_fork_entry finds the entry bad.
+MMR_HD int32_t page_fork_full(const PageState& st, const int32_t* parents, const int32_t* children, int32_t e) {
+  const int32_t parent = parents[e];
+  if (children[e] == MMR_PAGES_NONE || parent < 0 || parent >= st.S) return 0;
+  const int32_t l = st.lengths[parent];
+  return l < 0 || l > st.capacity ? 0 : static_cast<int32_t>(fdiv(static_cast<uint32_t>(l), st.div_T));
+}
+
+// The pages a fork shares, checked before anything is written: one entry a workgroup, in the launch before the plan.
+template <class X>
+MMR_HD void page_fork_check(X& x, const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children,
+                            int32_t n, uint32_t block, uint32_t blocks) {
+  uint32_t bad = 0;
+  for (int32_t e = static_cast<int32_t>(block); e < n; e += static_cast<int32_t>(blocks)) {
+    const int32_t full = page_fork_full(st, parents, children, e);
+    for (int32_t i = x.tid; i < full; i += X::kThreads) bad |= page_held(st, st.table[static_cast<int64_t>(parents[e]) * st.B + i]);
+  }
+  if (bad) x.atomic_or(&w.header[kPageForkBad], static_cast<int32_t>(bad));
+}
+
 // Entry e of fork: its flags; the parent's tokens and, where its last page is partly filled, that page.
 template <class X>
 MMR_HD uint32_t page_fork_entry(X& x, const PageState& st, const PageWork& w, int32_t parent, int32_t child, int32_t* len,
@@ -203,19 +238,29 @@ MMR_HD uint32_t page_fork_entry(X& x, const PageState& st, const PageWork& w, in
   const int32_t full = static_cast<int32_t>(fdiv(static_cast<uint32_t>(l), st.div_T));
   if (full * static_cast<int64_t>(st.T) != l) {
     const int32_t page = st.table[static_cast<int64_t>(parent) * st.B + full];
-    if (page < 0 || page >= st.P) flags |= MMR_PAGES_BAD_PAGE;
+    flags |= page_held(st, page);
     *src = page;
   }
   return flags;
 }
 
+// `prepared`: the launch before has scanned every segment and checked the shared pages; else the plan does it, place after
+// place of the parents' rows (n * B under 2^31).
 template <class X>
 MMR_HD void page_fork_plan(X& x, const PageState& st, const PageWork& w, int32_t* shared, const int32_t* parents,
-                           const int32_t* children, int32_t n) {
-  page_plan_scan(x, st, w, false);
+                           const int32_t* children, int32_t n, bool prepared = false) {
+  if (!prepared) page_plan_scan(x, st, w, false);
   const FreePages<X> pages(x, w, shared);
   int32_t fresh = 0;
   uint32_t bad = 0;
+  if (prepared) {
+    if (x.tid == 0) bad = static_cast<uint32_t>(x.atomic_exch(&w.header[kPageForkBad], 0));
+  } else {
+    for (int32_t at = x.tid; at < n * st.B; at += X::kThreads) {
+      const int32_t e = at / st.B, i = at - e * st.B;
+      if (i < page_fork_full(st, parents, children, e)) bad |= page_held(st, st.table[static_cast<int64_t>(parents[e]) * st.B + i]);
+    }
+  }
   for (int32_t base = 0; base < n; base += X::kThreads) {
     const int32_t e = base + x.tid;
     int32_t src = -1, len = 0;
@@ -238,7 +283,8 @@ MMR_HD void page_fork_plan(X& x, const PageState& st, const PageWork& w, int32_t
   page_verdict(x, w, bad, fresh, -1);
 }
 
-// Tables of the forked sequences; `block` of `blocks` workgroups share the entries.
+// Tables of the forked sequences; `block` of `blocks` workgroups share the entries.  The plan has checked the pages; they are
+// looked at again so that a table which is written while the call runs cannot lead out of refs.
 template <class X>
 MMR_HD void page_fork_rows(X& x, const PageState& st, const PageWork& w, const int32_t* parents, const int32_t* children,
                            int32_t n, uint32_t block, uint32_t blocks) {

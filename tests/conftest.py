@@ -42,8 +42,8 @@ def pytest_configure(config):
     if (_stale("tests/cpp/libmmr_emulation.so", cpp) or _stale("tests/cpp/hip_execute_context_test", cpp)
             or _stale("tests/cpp/libmmr_emulation_span_options.so", cpp)
             or _stale("tests/cpp/context_bench", cpp)
-            or (not gpu_only and (_stale("tests/cpp/sanitize_sweep", cpp) or _stale("tests/cpp/page_sweep", cpp)
-                                  or _stale("tests/cpp/page_sweep_threads", cpp)))) and (have_hipcc or not os.path.exists(
+            or (not gpu_only and any(_stale("tests/cpp/" + name, cpp) for name in (
+                "sanitize_sweep", "page_sweep", "page_sweep_threads", "page_faults", "page_faults_threads")))) and (have_hipcc or not os.path.exists(
                 os.path.join(ROOT, "tests", "cpp", "libmmr_emulation.so"))):
         subprocess.check_call(["bash", os.path.join(ROOT, "tests", "cpp", "build.sh")])
 

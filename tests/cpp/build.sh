@@ -44,3 +44,10 @@ echo "built ${here}/page_sweep"
 "${clang}" -O1 -g -std=c++20 -fsanitize=thread -Wall -Wextra -Wno-unknown-pragmas -I"${root}/include" \
   -I"${root}/multimesh-jax_amd/csrc" "${here}/page_sweep.cc" -pthread -o "${here}/page_sweep_threads"
 echo "built ${here}/page_sweep_threads"
+# The same routines on tables that are out of step with themselves.
+"${clang}" -O1 -g -std=c++20 -fsanitize=address,undefined -fno-sanitize-recover=undefined -fno-omit-frame-pointer -Wall -Wextra \
+  -Wno-unknown-pragmas -I"${root}/include" -I"${root}/multimesh-jax_amd/csrc" "${here}/page_faults.cc" -pthread -o "${here}/page_faults"
+echo "built ${here}/page_faults"
+"${clang}" -O1 -g -std=c++20 -fsanitize=thread -Wall -Wextra -Wno-unknown-pragmas -I"${root}/include" \
+  -I"${root}/multimesh-jax_amd/csrc" "${here}/page_faults.cc" -pthread -o "${here}/page_faults_threads"
+echo "built ${here}/page_faults_threads"
