@@ -62,7 +62,7 @@ struct PageWork {
   int32_t* len;   // per entry: tokens before the call
   int32_t* rank;  // per entry: first fresh page, -1 none
   PageMove* moves;
-  int32_t* map;  // which move of a compact takes a page
+  int32_t* map;  // which move of a compact takes a page, or brings one there
   int32_t n_segments;
 };
 
@@ -440,7 +440,7 @@ MMR_HD void page_compact_moves(const PageState& st, const PageWork& w, const Pag
   for (int32_t k = first; k < moves; k += step) {
     const int32_t dst = pages.kth_free(k), src = pages.kth_live(live - moves + k);
     w.moves[k] = PageMove{src, dst};
-    w.map[src] = k;
+    w.map[src] = w.map[dst] = k;
     st.refs[dst] = st.refs[src];
     st.refs[src] = 0;
   }
@@ -485,13 +485,15 @@ MMR_HD void page_compact_rows(X& x, const PageState& st, const PageWork& w, uint
       const int32_t page = row[i];
       if (page < 0 || page >= st.P) {
         bad |= MMR_PAGES_BAD_PAGE;
-      } else if (page >= live) {
-        // a page at or after `live` that was in use has moved; one that was not (a table out of step with the counts)
-        // has no new place, and what the map holds for it is left from an earlier call
-        const int32_t k = w.map[page];
-        if (k >= 0 && k < moves && w.moves[k].src == page) row[i] = w.moves[k].dst;
-        else bad |= MMR_PAGES_BAD_COUNT;
+        continue;
       }
+      // A page at or after `live` that was in use has moved, and every page before it that was not has been filled: a row
+      // that names one of these, or one behind `live` that did not move, is out of step with the counts.  What the map
+      // holds for a page without a move is left from an earlier call.
+      const int32_t k = w.map[page];
+      const PageMove mv = k >= 0 && k < moves ? w.moves[k] : PageMove{-1, -1};
+      if (mv.src == page) row[i] = mv.dst;
+      else if (mv.dst == page || page >= live) bad |= MMR_PAGES_BAD_COUNT;
     }
   }
   if (bad) x.atomic_or(&w.header[kPageStatus], static_cast<int32_t>(bad));

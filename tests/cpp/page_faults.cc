@@ -51,6 +51,13 @@ struct FaultCase {
     launch<K>(2, [&](Lanes<K>& x) { page_fork_rows(x, c.st, c.w, a.p, b.p, n, x.block, x.blocks); });
     c.move(rng);
   }
+  void compact(bool whole) {
+    scan(c, true);
+    launch<K>(1, [&](Lanes<K>& x) { page_compact_plan(x, c.st, c.w, shared.data(), whole); });
+    if (!whole) launch<8>(3, [&](Lanes<8>& x) { page_compact_list<Lanes<8>, kSegment>(x, c.st, c.w, shared.data()); });
+    launch<K>(3, [&](Lanes<K>& x) { page_compact_rows(x, c.st, c.w, x.block, x.blocks); });
+    c.move(rng);
+  }
 };
 
 // A fork whose parent's row names a page that is not there, or that nobody uses, changes nothing and says so.
@@ -89,11 +96,106 @@ void fork_cases(int32_t P, bool prepared) {
   f.expect("fork: a valid one beside bad rows", 0, m);
 }
 
+// A row that names a page nobody uses keeps that id through a compact, everything else moves, and the status tells.
+void compact_cases(int32_t P, bool whole) {
+  struct Fault {
+    int32_t id;
+    uint32_t flag;
+  };
+  // 7 pages are in use, so 0 .. 6 are live afterwards: pages 0, 2, 4 and 5 are given to the pages beyond
+  for (const Fault fault : {Fault{0, MMR_PAGES_BAD_COUNT}, Fault{4, MMR_PAGES_BAD_COUNT}, Fault{5, MMR_PAGES_BAD_COUNT},
+                            Fault{7, MMR_PAGES_BAD_COUNT}, Fault{P - 1, MMR_PAGES_BAD_COUNT}, Fault{P, MMR_PAGES_BAD_PAGE},
+                            Fault{-1, MMR_PAGES_BAD_PAGE}, Fault{6, 0}, Fault{P - 2, 0}}) {
+    FaultCase f(P, false);
+    f.holds(0, 14, {1, P - 2, 8, 3});
+    f.holds(3, 9, {P - 3, 6, P - 5});
+    f.compact(whole);  // so that what the calls below find from earlier ones is not zeros
+    if (f.c.status()) die("compact: a valid one");
+    for (size_t i = 0; i < f.c.table.n; ++i) f.c.table[i] = 0x7b7b7b7b;
+    for (int32_t i = 0; i < P; ++i) f.c.refs[i] = 0;
+    f.holds(0, 14, {1, P - 2, 8, 3});
+    f.holds(3, 9, {P - 3, 6, P - 5});
+    f.c.lengths[5] = 4;
+    f.at(5, 0) = fault.id;
+    Model m = f.c.snapshot();
+    int32_t& id = m.table[5 * static_cast<size_t>(f.c.B)];
+    if (fault.flag == MMR_PAGES_BAD_PAGE) id = 0;
+    model_compact(f.c, &m);
+    if (fault.flag) id = fault.id;
+    f.compact(whole);
+    f.expect("compact: a row in error", fault.flag, m);
+  }
+}
+
+// What free takes from a row in error, beside what is right.
+void free_cases(int32_t P) {
+  auto run = [&](FaultCase& f, const std::vector<int32_t>& a) {
+    Exact<int32_t> ids(a.size());
+    std::copy(a.begin(), a.end(), ids.p);
+    launch<K>(static_cast<uint32_t>(a.size()), [&](Lanes<K>& x) { page_free(x, f.c.st, f.c.w, f.shared.data(), ids.p); });
+  };
+  for (const int32_t bad : {-1, P, 2147483647}) {
+    FaultCase f(P, false);
+    f.holds(2, 12, {4, 9, 6});
+    f.c.refs[9] = 0;
+    f.at(2, 1) = bad;
+    Model m = f.c.snapshot();
+    m.lengths[2] = m.refs[4] = m.refs[6] = 0;
+    run(f, {2, 2});
+    f.expect("free: an id outside the pool", MMR_PAGES_BAD_PAGE, m);
+  }
+  for (const int32_t users : {0, -3}) {
+    FaultCase f(P, false);
+    f.holds(2, 12, {4, 9, 6});
+    f.c.refs[9] = users;
+    Model m = f.c.snapshot();
+    m.lengths[2] = m.refs[4] = m.refs[6] = 0;
+    run(f, {2});
+    f.expect("free: a page that nobody uses", MMR_PAGES_BAD_COUNT, m);
+  }
+  FaultCase f(P, false);  // three rows name page 9, which has two users
+  f.holds(2, 12, {4, 9, 6});
+  f.holds(1, 6, {9, 7});
+  f.holds(0, 2, {9});
+  f.c.refs[9] = 2;
+  Model m = f.c.snapshot();
+  for (int32_t page : {4, 9, 6, 7}) m.refs[page] = 0;
+  for (int32_t s : {0, 1, 2}) m.lengths[s] = 0;
+  run(f, {0, 1, 2});
+  f.expect("free: more rows than users", MMR_PAGES_BAD_COUNT, m);
+}
+
+// An extend into a partly filled page that is not there, or whose only user is not this sequence.
+void extend_cases(int32_t P) {
+  struct Fault {
+    int32_t id, users;
+    uint32_t flag;
+  };
+  for (const Fault fault : {Fault{-1, 1, MMR_PAGES_BAD_PAGE}, Fault{P, 1, MMR_PAGES_BAD_PAGE}, Fault{9, 0, MMR_PAGES_SHARED_TAIL},
+                            Fault{9, 2, MMR_PAGES_SHARED_TAIL}}) {
+    FaultCase f(P, false);
+    f.holds(2, 6, {4, 9});
+    f.c.refs[9] = fault.users;
+    f.at(2, 1) = fault.id;
+    const Model m = f.c.snapshot();
+    Exact<int32_t> a(2), b(2);
+    a[0] = 0, b[0] = 5, a[1] = 2, b[1] = 1;
+    scan(f.c, false);
+    launch<K>(1, [&](Lanes<K>& x) { page_extend_plan(x, f.c.st, f.c.w, f.shared.data(), a.p, b.p, 2, true); });
+    f.expect("extend: a bad last page", fault.flag, m);
+  }
+}
+
 }  // namespace
 
 int main() {
   for (const int32_t P : {24, 3 * kSegment + 9})
-    for (const bool prepared : {false, true}) fork_cases(P, prepared);
+    for (const bool form : {false, true}) {
+      fork_cases(P, form);
+      compact_cases(P, form);
+      free_cases(P);
+      extend_cases(P);
+    }
   std::printf("OK\n");
   return 0;
 }

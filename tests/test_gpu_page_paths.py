@@ -42,3 +42,59 @@ def test_a_fork_of_a_bad_row_changes_nothing(ctx, form, page, id, users, flag): 
     p.op("fork", [0, 1, 0], [3, 4, 5])  # and nothing of the refusal is left
     p.check()
     p.close()
+
+
+# a compact of more than 16,384 pages lists its moves in a launch of its own, one of more than 8,192 scans in one
+@pytest.mark.parametrize("P", [24, 9001, 20001])
+@pytest.mark.parametrize("id,flag", [(0, "BAD_COUNT"), (5, "BAD_COUNT"), (7, "BAD_COUNT"), ("last", "BAD_COUNT"), ("P", "BAD_PAGE"), (-1, "BAD_PAGE")])
+def test_a_compact_keeps_a_bad_id_and_tells(ctx, P, id, flag):  # noqa: F811
+    """A row names a page that is not there, or that nobody uses, before and behind the pages in use."""
+    say("compact of a bad row, %d pages: %s" % (P, id))
+    p = Pair(ctx, S=8, Bl=6, P=P, T=4, shape=(4, 2, 8), type="BF16", seed=9)
+    m = p.model
+    for s, n, row in ((0, 14, [1, P - 2, 8, 3]), (3, 9, [P - 3, 6, P - 5]), (5, 4, [2])):
+        m.lengths[s], m.table[s, :len(row)] = n, row
+        m.refs[row] += 1
+    for name in ("table", "lengths", "refs"):
+        put(p, name)
+    p.op("compact")
+    p.check()
+    m.refs[m.table[5, 0]] = 0  # sequence 5 names what is no longer its own
+    for s, n, row in ((0, 14, [1, P - 2, 8, 3]), (3, 9, [P - 3, 6, P - 5])):
+        m.table[s, :len(row)] = row
+    m.refs[:] = 0
+    m.refs[m.table[0, :4]] += 1
+    m.refs[m.table[3, :3]] += 1  # 7 pages in use
+    bad = {"P": P, "last": P - 1}.get(id, id)
+    m.table[5, 0] = bad
+    for name in ("table", "refs"):
+        put(p, name)
+    m.table[5, 0] = 0
+    p.op("compact")
+    m.table[5, 0] = bad
+    assert p.cache.Status() == ([flag], 7)
+    p.check()
+    p.close()
+
+
+def test_a_free_of_rows_out_of_step(ctx):  # noqa: F811
+    """An id outside, a page that nobody uses, a page that more rows name than use it: told, and no count below zero."""
+    p = Pair(ctx, S=8, Bl=6, P=24, T=4, shape=(4, 2, 8), type="BF16", seed=9)
+    m = p.model
+    p.op("extend", [0, 1, 2, 3], [8, 9, 12, 5])
+    row = m.table.copy()
+    m.table[0, 1] = 24
+    m.refs[row[1, 0]] = 0
+    m.table[2, 2] = m.table[3, 0]
+    for name in ("table", "refs"):
+        put(p, name)
+    for seqs, flag in (([0], "BAD_PAGE"), ([1], "BAD_COUNT"), ([2, 3], "BAD_COUNT")):
+        p.cache.Free(p.ids(seqs))
+        for s in seqs:
+            for page in m.table[s, :m.blocks(m.lengths[s])]:
+                if page < 24 and m.refs[page] > 0:
+                    m.refs[page] -= 1
+            m.lengths[s] = 0
+        assert p.cache.Status() == ([flag], int((m.refs > 0).sum()))
+        p.check()
+    p.close()
