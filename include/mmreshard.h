@@ -604,7 +604,8 @@ int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* options, mmr_r
 int mmr_rotary_destroy(mmr_rotary* rotary);
 
 /* out := x with its rows turned.  x and out: F32, BF16 or F16, rank 2 to 4, of one descriptor (out may be x itself, and
- * overlaps it in no other way); the last dim is the row, unsharded and minor-most, at least rotary_dim long, the rest of
+ * overlaps it in no other way; replicas of out may be adopted in one buffer, which is written once, and its tiles overlap in
+ * no other way, which is refused); the last dim is the row, unsharded and minor-most, at least rotary_dim long, the rest of
  * it passes through.  Every other dim may be sharded, padded and laid out at will; padding is left alone.  The position
  * of a row is offset + its index along seq_dim in the whole array, wherever its tile is, or what `positions` holds: an
  * S32 store [sequence], or [dim 0, sequence], whose tile on every device covers the sequence of x's tile there (sharded

@@ -212,6 +212,7 @@ struct mmr_store {
   size_t bytes = 0;
   std::vector<char*> adopted;  // caller-owned buffers, one per device (mmr_store_adopt)
   char* host = nullptr;        // pinned host copy while the store is offloaded (the device buffers are gone then)
+  bool tiles_overlap = false;  // of adopted buffers: the caller has put some over one another
   bool watched = false;        // another operator's handle keeps this store's addresses
   mmr_context* owner = nullptr;
 
@@ -1292,6 +1293,7 @@ const mmr_sharded_shape& store_shape(const mmr_store* store) { return store->sha
 const std::string& store_key(const mmr_store* store) { return store->shape_key; }
 int64_t store_ordinal(const mmr_store* store) { return store->ordinal; }
 char* store_tile(const mmr_store* store, int64_t k) { return store->tile(k); }
+bool store_tiles_overlap(const mmr_store* store) { return store->tiles_overlap; }
 
 }  // namespace mmr
 
@@ -1706,6 +1708,9 @@ int mmr_store_adopt(mmr_context* ctx, const mmr_sharded_shape* shape, const char
       return fail(MMR_INVALID_ARGUMENT, "buffer of device %lld is not 16-byte aligned", (long long)(s->side.dev_start + k));
     s->adopted.push_back(static_cast<char*>(device_ptrs[k]));
   }
+  std::vector<char*> sorted = s->adopted;
+  std::sort(sorted.begin(), sorted.end());
+  for (size_t k = 1; k < sorted.size(); ++k) s->tiles_overlap |= sorted[k] - sorted[k - 1] < s->side.shard_bytes;
   s->shape = *shape;
   s->shape_key = mmr::descriptor_key(*shape);
   s->name = name ? name : "anonymous";

@@ -54,6 +54,7 @@ const mmr_sharded_shape& store_shape(const mmr_store* store);
 const std::string& store_key(const mmr_store* store);
 int64_t store_ordinal(const mmr_store* store);
 char* store_tile(const mmr_store* store, int64_t k);
+bool store_tiles_overlap(const mmr_store* store);  // adopted buffers that lie over one another, as replicas in one do
 
 }  // namespace mmr
 

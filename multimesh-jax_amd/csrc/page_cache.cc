@@ -162,6 +162,32 @@ int64_t tile_valid(const Side& s, int64_t k, int i) {
   return std::max<int64_t>(0, std::min(s.ext[i], s.size[i] - tile_start(s, k, i)));
 }
 
+bool tile_empty(const Side& s, int64_t k) {
+  for (int i = 0; i < s.rank; ++i)
+    if (tile_valid(s, k, i) == 0) return true;
+  return false;
+}
+
+// Replicas that the caller keeps in one buffer are turned once: *again says that an earlier device than k writes k's tile.
+// Tiles that lie over one another in any other way are refused, as their writes have no order.
+int check_again(const mmr_store* out, int64_t k, bool* again) {
+  *again = false;
+  if (!mmr::store_tiles_overlap(out)) return MMR_OK;
+  const Side& s = mmr::store_side(out);
+  const char* mine = mmr::store_tile(out, k);
+  for (int64_t m = 0; m < k; ++m) {
+    const char* other = mmr::store_tile(out, m);
+    if (mine + s.shard_bytes <= other || other + s.shard_bytes <= mine || tile_empty(s, m)) continue;
+    bool same = mine == other;
+    for (int i = 0; i < s.rank; ++i) same &= tile_at(s, k, i) == tile_at(s, m, i);
+    if (!same)
+      return fail(MMR_INVALID_ARGUMENT, "the buffers of devices %lld and %lld of the output store overlap", (long long)(s.dev_start + m),
+                  (long long)(s.dev_start + k));
+    *again = true;
+  }
+  return MMR_OK;
+}
+
 int check_row(const Side& s, const char* what) {
   const int d = s.rank - 1;
   if (s.tiles[d] != 1) return fail(MMR_INVALID_ARGUMENT, "the last dim of the %s store is sharded", what);
@@ -600,6 +626,9 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
                     (long long)(s.dev_start + k));
       b.positions = reinterpret_cast<const int32_t*>(mmr::store_tile(positions, k)) + first;
     }
+    bool again = false;
+    if (int rc = check_again(out, k, &again)) return rc;
+    if (again) continue;
     in_place &= b.src == b.dst;
     l.buffers.push_back(b);
   }
@@ -642,7 +671,7 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
   };
   auto add = [&](const mmr_store* s, const Side* pool, const std::vector<char*>* pool_tiles, const mmr_store* out, bool turn) {
     const Side& d = mmr::store_side(s);
-    if (d.size[0] == 0 || d.size[1] == 0) return;
+    if (d.size[0] == 0 || d.size[1] == 0) return static_cast<int>(MMR_OK);
     mmr::RotaryShape j{};
     j.tokens = j.seq = static_cast<uint32_t>(d.size[0]);
     j.heads = static_cast<uint32_t>(d.ext[1]);
@@ -663,11 +692,16 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
       b.outer = 1, b.seq = j.seq, b.heads = static_cast<uint32_t>(tile_valid(d, dev, 1));
       b.shape = static_cast<uint32_t>(l.shapes.size());
       if (b.heads == 0) continue;
+      bool again = false;
+      if (out)
+        if (int rc = check_again(out, dev, &again)) return rc;
+      if (again) continue;
       in_place &= b.src == b.dst;
       l.buffers.push_back(b);
     }
     l.shapes.push_back(j);
     rows.push_back(Row{d.size[2], turn, in_place});
+    return static_cast<int>(MMR_OK);
   };
   auto add_pool = [&](const mmr_store* s, int32_t pool, bool turn, const char* what) {
     if (int rc = check_new(s, what)) return rc;
@@ -686,8 +720,7 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
         return fail(MMR_INVALID_ARGUMENT, "the heads of the %s store and of pool %d are sharded differently", what, pool);
     if (turn)
       if (int rc = check_rotary(ctx, rotary, d.size[2], d.dtype)) return rc;
-    add(s, &p, &pages->pools[static_cast<size_t>(pool)].tiles, nullptr, turn);
-    return static_cast<int>(MMR_OK);
+    return add(s, &p, &pages->pools[static_cast<size_t>(pool)].tiles, nullptr, turn);
   };
   if (q) {
     if (int rc = check_new(q, "q")) return rc;
@@ -695,7 +728,7 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
     if (q != q_out && mmr::store_key(q) != mmr::store_key(q_out))
       return fail(MMR_INVALID_ARGUMENT, "q and q_out have different descriptors");
     if (int rc = check_rotary(ctx, rotary, mmr::store_side(q).size[2], dtype)) return rc;
-    add(q, nullptr, nullptr, q_out, true);
+    if (int rc = add(q, nullptr, nullptr, q_out, true)) return rc;
   }
   if (int rc = add_pool(k, k_pool, rotary != nullptr, "k")) return rc;
   if (v)

@@ -3,7 +3,10 @@ chunks), on both sides of each limit, and on tables that are out of step with th
 import numpy as np
 import pytest
 
-from test_gpu_pages import Pair, ctx, say  # noqa: F401  (ctx is the fixture)
+import multimesh_jax_amd as mm
+
+import page_model as pm
+from test_gpu_pages import Pair, compare, ctx, say, split, values, whole  # noqa: F401  (ctx is the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +101,78 @@ def test_a_free_of_rows_out_of_step(ctx):  # noqa: F811
         assert p.cache.Status() == ([flag], int((m.refs > 0).sum()))
         p.check()
     p.close()
+
+
+def adopted(c, type, shape, values, devices):
+    """A store of `shape` whose devices[i] is the row of `values` that device i holds, every row in one buffer however many
+    devices share it -> (the store, the store that owns the buffers)."""
+    raw = np.ascontiguousarray(values)
+    own = whole(c, raw.view(np.uint8).reshape(len(raw), -1), "U8")
+    at, size = c.SliceLocalShard(0, own), raw[0].nbytes
+    assert size % 16 == 0
+    return c.AdoptShards(shape, [at + size * d for d in devices]), own
+
+
+@pytest.mark.parametrize("replicas_major", [False, True])
+@pytest.mark.parametrize("R,interleaved", [(16, False), (10, True)])
+def test_replicas_in_one_buffer_are_turned_once(ctx, replicas_major, R, interleaved):  # noqa: F811
+    """Two halves of a sequence on two devices each, both in the buffer of the half; in place, and into such a store."""
+    rng = np.random.Generator(np.random.PCG64(5))
+    digits = [(3, 1, 0), (14, 2, 1), (16, 1, 2), (1, 2, 3)] if not replicas_major else [(3, 1, 1), (14, 2, 2), (16, 1, 3), (1, 2, 0)]
+    shape = mm.sharded_shape("BF16", digits, 0, 4)
+    half_of = [0, 0, 1, 1] if not replicas_major else [0, 1, 0, 1]
+    x = values(rng, (3, 14, 16), "BF16")
+    halves = np.stack([x[:, :7], x[:, 7:]])
+    sx, own = adopted(ctx, "BF16", shape, halves, half_of)
+    so, own2 = adopted(ctx, "BF16", shape, np.zeros_like(halves), half_of)
+    plan = ctx.CreateRotary(R, interleaved=interleaved, magnitude=1.5)
+    ctx.ApplyRotary(plan, sx, so, seq_dim=1, offset=9)
+    ctx.ApplyRotary(plan, sx, seq_dim=1, offset=9)
+    want, size = pm.turn(pm.from_bits(x, "BF16"), 9 + np.arange(14)[None, :], pm.frequencies(R), interleaved, 1.5)
+    for o in (own2, own):
+        got = ctx.ReadShard(o, 0, np.uint16).reshape(halves.shape)
+        got = np.concatenate([got[0], got[1]], 1)
+        compare(got, want, size, "BF16", 1.5)
+        assert np.array_equal(got[..., R:], x[..., R:])
+    plan.Destroy()
+    for s in (sx, so, own, own2):
+        ctx.Free(s)
+
+
+def test_queries_of_replicas_in_one_buffer_are_turned_once(ctx):  # noqa: F811
+    p = Pair(ctx, S=4, Bl=4, P=16, T=4, shape=(4, 2, 16), type="BF16", n_pools=1, n_dev=2, cut=2, seed=3)
+    p.op("extend", [2, 0], [5, 3])
+    rng = np.random.Generator(np.random.PCG64(3))
+    k, q = values(rng, (8, 2, 16), "BF16"), values(rng, (1, 8, 3, 16), "BF16")
+    sq, own = adopted(ctx, "BF16", mm.sharded_shape("BF16", [(8, 1, 0), (3, 1, 1), (16, 1, 2), (1, 3, 3)], 0, 3), q, [0, 0, 0])
+    plan = ctx.CreateRotary(16)
+    p.cache.Write(p.ids([2, 0]), p.ids([0, 5, 8]), 0, split(ctx, k, "BF16", 1, 2), rotary=plan, q=sq, q_out=sq)
+    position = np.append(np.arange(5), np.arange(3))
+    want, size = pm.turn(pm.from_bits(q[0], "BF16"), position[:, None], pm.frequencies(16))
+    compare(ctx.ReadShard(own, 0, np.uint16).reshape(8, 3, 16), want, size, "BF16")
+    assert p.cache.Status() == ([], 3)
+    p.close()
+
+
+def test_tiles_that_lie_over_one_another_are_refused(ctx):  # noqa: F811
+    """Two parts of an array in one buffer, or replicas that do not begin together, as a result or in place."""
+    own = whole(ctx, np.zeros(4096, np.uint8), "U8")
+    at = ctx.SliceLocalShard(0, own)
+    parts = mm.sharded_shape("BF16", [(6, 2, 0), (2, 1, 1), (16, 1, 2)], 0, 2)     # 192 bytes each
+    copies = mm.sharded_shape("BF16", [(3, 1, 0), (2, 1, 1), (16, 1, 2), (1, 2, 3)], 0, 2)
+    plan = ctx.CreateRotary(16)
+    ctx.Sync()
+    launches = ctx.stats["kernel_launches"]
+    for shape, ptrs in ((parts, [at, at]), (parts, [at, at + 176]), (copies, [at, at + 16]), (copies, [at + 176, at])):
+        s = ctx.AdoptShards(shape, ptrs)
+        apart = ctx.AdoptShards(shape, [at + 1024, at + 1024 + 192])
+        for x in (s, apart):
+            with pytest.raises(mm.MmrError, match="overlap") as e:
+                ctx.ApplyRotary(plan, x, s, seq_dim=0)
+            assert e.value.status_name == "INVALID_ARGUMENT"
+        assert ctx.stats["kernel_launches"] == launches
+        ctx.ApplyRotary(plan, s, apart, seq_dim=0)  # only read
+        launches = ctx.stats["kernel_launches"]
+        ctx.Free(s)
+        ctx.Free(apart)
+    plan.Destroy()
