@@ -620,7 +620,7 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
  * are those of a sequence MMR_PAGES_NONE; the sequences are distinct (of two entries of one, either may be kept).  k
  * goes to pool k_pool, v (or NULL) to pool v_pool: stores [tokens, heads, dim], heads sharded as in the pool.  With a
  * rotary plan k is turned on its way, and q (any heads, [tokens, heads, dim], or NULL) is turned into q_out (or in
- * place).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.  Tokens of an entry whose
+ * place; q_out and the pools overlap nothing else that the call reads or writes, so q_out is not k or v).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.  Tokens of an entry whose
  * sequence or page is not there, or that are more than the sequence holds, are left out (q_out too), the others are
  * written; the reason is kept for mmr_pages_status. */
 int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* begins, int32_t n, int32_t k_pool, mmr_store* k,

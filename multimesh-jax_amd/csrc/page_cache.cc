@@ -727,6 +727,7 @@ int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* b
     if (int rc = mmr::context_check_store(ctx, q_out, "q_out")) return rc;
     if (q != q_out && mmr::store_key(q) != mmr::store_key(q_out))
       return fail(MMR_INVALID_ARGUMENT, "q and q_out have different descriptors");
+    if (q_out == k || q_out == v) return fail(MMR_INVALID_ARGUMENT, "q_out is also the %s store", q_out == k ? "k" : "v");
     if (int rc = check_rotary(ctx, rotary, mmr::store_side(q).size[2], dtype)) return rc;
     if (int rc = add(q, nullptr, nullptr, q_out, true)) return rc;
   }

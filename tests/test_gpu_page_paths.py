@@ -176,3 +176,22 @@ def test_tiles_that_lie_over_one_another_are_refused(ctx):  # noqa: F811
         ctx.Free(s)
         ctx.Free(apart)
     plan.Destroy()
+
+
+def test_queries_are_not_turned_into_the_keys_or_values(ctx):  # noqa: F811
+    """They are read while the queries are written."""
+    p = Pair(ctx, S=4, Bl=4, P=16, T=4, shape=(4, 2, 16), type="BF16", seed=3)
+    p.op("extend", [2], [5])
+    k, v = (split(ctx, values(np.random.Generator(np.random.PCG64(s)), (5, 2, 16), "BF16"), "BF16", 1, 1) for s in range(2))
+    plan = ctx.CreateRotary(16)
+    ctx.Sync()
+    launches = ctx.stats["kernel_launches"]
+    for q, q_out, what in ((k, k, "k"), (v, k, "k"), (v, v, "v"), (k, v, "v")):
+        ids = p.ids([2]), p.ids([0, 5])
+        with pytest.raises(mm.MmrError, match="q_out is also the %s store" % what) as e:
+            p.cache.Write(*ids, 0, k, 1, v, rotary=plan, q=q, q_out=q_out)
+        assert e.value.status_name == "INVALID_ARGUMENT"
+    assert ctx.stats["kernel_launches"] == launches
+    p.check()
+    plan.Destroy()
+    p.close()
