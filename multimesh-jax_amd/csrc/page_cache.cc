@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <limits>
 #include <new>
 #include <set>
 #include <vector>
@@ -489,7 +490,8 @@ int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* o, mmr_rotary*
   if (o->rotary_dim < 2 || o->rotary_dim % 2 || o->rotary_dim > (1 << 20))
     return fail(MMR_INVALID_ARGUMENT, "rotary dim %d is not even and in [2, 2^20]", o->rotary_dim);
   if (!o->frequencies && !(o->base > 0 && std::isfinite(o->base))) return fail(MMR_INVALID_ARGUMENT, "base %g", o->base);
-  if (!(o->magnitude >= 0 && std::isfinite(o->magnitude))) return fail(MMR_INVALID_ARGUMENT, "magnitude %g", o->magnitude);
+  // held in 32 bits
+  if (!(o->magnitude >= 0 && o->magnitude <= std::numeric_limits<float>::max())) return fail(MMR_INVALID_ARGUMENT, "magnitude %g", o->magnitude);
   if (o->scaling < MMR_ROTARY_UNSCALED || o->scaling > MMR_ROTARY_BY_PARTS)
     return fail(MMR_INVALID_ARGUMENT, "scaling %d", o->scaling);
   if (o->scaling != MMR_ROTARY_UNSCALED && !(o->factor > 0 && std::isfinite(o->factor)))

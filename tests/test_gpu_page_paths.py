@@ -195,3 +195,12 @@ def test_queries_are_not_turned_into_the_keys_or_values(ctx):  # noqa: F811
     p.check()
     plan.Destroy()
     p.close()
+
+
+@pytest.mark.parametrize("magnitude", [3.5e38, 1e300, -1.0, float("nan")])
+def test_magnitudes_that_32_bits_do_not_hold_are_refused(ctx, magnitude):  # noqa: F811
+    with pytest.raises(mm.MmrError, match="magnitude") as e:
+        ctx.CreateRotary(8, magnitude=magnitude)
+    assert e.value.status_name == "INVALID_ARGUMENT"
+    ctx.CreateRotary(8, magnitude=3.4e38).Destroy()
+    ctx.CreateRotary(8, magnitude=0.0).Destroy()
