@@ -6,6 +6,7 @@ import pytest
 import multimesh_jax_amd as mm
 
 import page_model as pm
+import test_gpu_pages as base
 from test_gpu_pages import Pair, compare, ctx, say, split, values, whole  # noqa: F401  (ctx is the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -204,3 +205,185 @@ def test_magnitudes_that_32_bits_do_not_hold_are_refused(ctx, magnitude):  # noq
     assert e.value.status_name == "INVALID_ARGUMENT"
     ctx.CreateRotary(8, magnitude=3.4e38).Destroy()
     ctx.CreateRotary(8, magnitude=0.0).Destroy()
+
+
+# ---------------------------------------------------------------- forms of the launches
+
+def test_extend_in_two_launches(ctx):  # noqa: F811
+    """More than 16,384 pages may be given out, so the tables are written by a launch of their own where it is more than
+    4,096 pages, by the plan where it is not; too few pages for all, and a bad entry, change nothing."""
+    p = Pair(ctx, S=6000, Bl=8, P=40000, T=4, shape=(4, 1, 4), type="U8", n_pools=1, seed=3)
+    m, rng = p.model, np.random.Generator(np.random.PCG64(3))
+    some = rng.permutation(6000)
+    p.op("extend", some[:2500], rng.integers(0, 16, 2500))       # about 5,000 pages, in five segments and more
+    p.check()
+    p.op("free", some[:2500:3])
+    p.op("extend", some[:5000], rng.integers(0, 16, 5000))       # more sequences than the launch has workgroups
+    assert (m.refs > 0).sum() > 12000
+    p.check()
+    p.op("extend", rng.permutation(6000), np.ones(6000, int))    # a step of decoding: under 4,096 fresh pages
+    p.check()
+    for seqs, counts, flag in ((np.arange(6000), np.full(6000, 32) - m.lengths, "OUT_OF_PAGES"),
+                               (np.append(np.arange(4000), 7), np.full(4001, 1), "REPEATED")):
+        p.cache.Extend(p.ids(seqs), p.ids(counts))
+        assert p.cache.Status() == ([flag], int((m.refs > 0).sum()))
+        p.check()
+    p.op("extend", [int(np.argmin(m.lengths))], [5])
+    p.check()
+    p.close()
+
+
+def test_fork_and_compact_of_more_sequences_than_workgroups(ctx):  # noqa: F811
+    p = Pair(ctx, S=11000, Bl=6, P=30000, T=4, shape=(4, 1, 5), type="U8", n_pools=2, seed=4)
+    m, rng = p.model, np.random.Generator(np.random.PCG64(4))
+    p.op("extend", np.arange(5000), rng.integers(0, 21, 5000))
+    p.op("fork", rng.integers(0, 5000, 5500), 5000 + rng.permutation(6000)[:5500])
+    p.check()
+    p.op("free", rng.permutation(11000)[:6000])
+    p.op("compact")  # lists its moves in a launch of its own
+    p.check()
+    p.close()
+
+
+# page, as (tokens, rest): one of 14 pieces in a pool's buffer is more than 64 pairs may check in one launch
+COPIES = {"few pairs of long pages": (140, (4, 7000, 2), 64), "by destination": (600, (4, 3), 100), "in the given order": (3000, (4, 3), 100),
+          "by destination, more than one round": (9000, (4, 8), 3000), "in the given order, more than one round": (20000, (4, 8), 2000)}
+
+
+@pytest.mark.parametrize("name", COPIES)
+def test_copies_that_are_planned(ctx, name):  # noqa: F811
+    """Copies that one launch does not check: results, entries that are none or copy a page onto itself, refusals."""
+    P, shape, n = COPIES[name]
+    p = Pair(ctx, S=4, Bl=4, P=P, T=4, shape=shape, type="U8", n_pools=2, seed=5)
+    rng = np.random.Generator(np.random.PCG64(5))
+    say("planned copy, " + name)
+    ids = rng.permutation(P)
+    dst, src = ids[:n], rng.choice(ids[n:], n)
+    a, b = p.ids(src), p.ids(dst)
+    before = ctx.stats["kernel_launches"]
+    p.cache.Copy(a, b)
+    p.model.copy(src, dst)
+    assert ctx.stats["kernel_launches"] == before + 2  # the plan and the move
+    p.check()
+    src[3], dst[5], src[5] = dst[3], -1, P + 7  # onto itself; no entry
+    p.cache.Copy(p.ids(src), p.ids(dst))
+    on = dst >= 0
+    p.model.copy(src[on], dst[on])
+    p.check()
+    for at, (s, d), flag in ((9, (src[9], dst[10]), "REPEATED"), (9, (dst[20], dst[9]), "OVERLAP"), (n - 1, (src[0], P), "BAD_PAGE"),
+                             (0, (-1, dst[0]), "BAD_PAGE"), (n // 2, (P, dst[n // 2]), "BAD_PAGE")):
+        a, b = src.copy(), dst.copy()
+        a[at], b[at] = s, d
+        p.cache.Copy(p.ids(a), p.ids(b))
+        assert p.cache.Status() == ([flag], 0)
+        p.check()
+    p.op("copy", src[on][::-1].copy(), dst[on][::-1].copy())  # and no mark is left
+    p.check()
+    p.close()
+
+
+@pytest.mark.parametrize("bytes", [20000, 20007, 8192, 8200])
+def test_pages_of_several_pieces_beside_small_ones(ctx, bytes):  # noqa: F811
+    """Fork, copy (in one launch and planned) and compact of pools whose pages are more than one 8-KiB piece, with a pool of
+    small pages in the same cache."""
+    P, T = 90, 1
+    p = Pair(ctx, S=20, Bl=8, P=P, T=T, shape=(T, bytes), type="U8", n_pools=2, seed=6)
+    rng = np.random.Generator(np.random.PCG64(6))
+    p.cache.Destroy()
+    for size in (48, 7):
+        small = rng.integers(0, 256, (P, T, size), dtype=np.uint8)
+        p.model.pools.append(small)
+        p.pools.append(split(ctx, small.copy(), "U8", 1, 1))
+    p.cache = ctx.CreatePages(p.pools, p.table, p.lengths, p.refs, page_tokens=T)
+    m = p.model
+    p.op("extend", [0, 1, 2], [8, 5, 7])
+    p.op("copy", [0, 9, 12], [60, 70, 89])
+    p.check()
+    p.op("copy", np.arange(20).repeat(4)[:70], 20 + np.arange(70))
+    p.check()
+    p.op("fork", [1, 1, 0], [4, 5, 6])
+    p.op("free", [0, 1])
+    p.op("compact")
+    p.check()
+    p.close()
+    # partly filled pages: a fork copies one a child
+    p = Pair(ctx, S=9, Bl=4, P=30, T=3, shape=(3, bytes), type="U8", n_pools=1, seed=7)
+    p.op("extend", [0, 1], [8, 4])
+    p.op("fork", [0, 1, 1], [4, 5, 6])
+    p.check()
+    p.close()
+
+
+def test_more_pieces_than_workgroups(ctx):  # noqa: F811
+    """264,000 pieces; a launch has 262,144 workgroups, which then loop."""
+    P, n, words = 66000, 33000, 129 * 4
+    page = lambda i: (np.arange(P * words, dtype=np.uint32) * np.uint32(2654435761) + np.uint32(i * 977)).reshape(P, 1, words)  # noqa: E731
+    pools = []
+    for i in range(8):
+        pools.append(split(ctx, page(i), "U32", 1, 1))
+    tables = [whole(ctx, np.zeros(s, np.int32)) for s in ((4, 4), (4,), (P,))]
+    cache = ctx.CreatePages(pools, *tables, page_tokens=1)
+    rng = np.random.Generator(np.random.PCG64(8))
+    ids = rng.permutation(P).astype(np.int32)
+    say("a copy of 264,000 pieces")
+    cache.Copy(whole(ctx, ids[:n]), whole(ctx, ids[n:]))
+    assert cache.Status() == ([], 0)
+    for i, s in enumerate(pools):
+        want = page(i)
+        want[ids[n:]] = want[ids[:n]]
+        assert np.array_equal(ctx.ReadShard(s, 0, np.uint32).reshape(want.shape), want)
+    cache.Destroy()
+    for s in pools + tables:
+        ctx.Free(s)
+    ctx.ClearStoreCache()
+
+
+def turned(ctx, case, backward, seed, launches=None):  # noqa: F811
+    shape, seq_dim, cut, n_dev, layout, R, interleaved, type, scaling, magnitude, offset = case
+    rng = np.random.Generator(np.random.PCG64(seed))
+    x = values(rng, shape, type)
+    sx, out = split(ctx, x, type, cut, n_dev, layout), split(ctx, np.zeros_like(x), type, cut, n_dev, layout)
+    more, freq = dict(scaling), None
+    if more.pop("frequencies", False):
+        more["frequencies"] = rng.uniform(-2, 2, R // 2)
+        freq = more["frequencies"].astype(np.longdouble)
+    plan = ctx.CreateRotary(R, interleaved=interleaved, magnitude=magnitude, **more)
+    before = ctx.stats["kernel_launches"]
+    ctx.ApplyRotary(plan, sx, out, seq_dim=seq_dim, offset=offset, backward=backward)
+    assert launches is None or ctx.stats["kernel_launches"] == before + launches
+    place = [1] * (len(shape) - 1)
+    place[seq_dim] = shape[seq_dim]
+    got = base.joined(ctx, out, x, cut, n_dev, layout)[0]
+    want, size = pm.turn(pm.from_bits(x, type), (offset + np.arange(shape[seq_dim])).reshape(place),
+                         pm.frequencies(R, **scaling) if freq is None else freq, interleaved, magnitude, backward)
+    compare(got, want, size, type, magnitude)
+    assert np.array_equal(got[..., R:], x[..., R:])
+    plan.Destroy()
+    for s in (sx, out):
+        ctx.Free(s)
+
+
+@pytest.mark.parametrize("i", range(len(base.ROTARY)))
+def test_rotary_positions_of_fixed_values(ctx, i):  # noqa: F811
+    turned(ctx, base.ROTARY[i], i % 2 == 1, 100 + i)
+
+
+@pytest.mark.parametrize("n_dev,launches", [(8, 1), (9, 1), (24, 1), (25, 2), (60, 3)])
+@pytest.mark.parametrize("type,R", [("BF16", 16), ("F32", 6)])
+def test_rotary_positions_on_many_devices(ctx, n_dev, launches, type, R):  # noqa: F811
+    """A launch takes 24 buffers."""
+    turned(ctx, ((n_dev * 3 - 2, 3, 16), 0, 0, n_dev, None, R, False, type, {}, 1.0, 5), False, n_dev, launches)
+
+
+MIXED = [
+    (2, 4, 32, 32, False, "BF16", 1, None, 16, [512] + [1] * 300),              # a prompt beside a step of decoding
+    (2, 4, 32, 16, True, "F16", 2, None, 8, [1] * 90 + [70, 1, 1, 0, 33] + [1] * 90),
+    (9, 9, 16, 16, False, "F32", 9, None, 4, [5, 1, 1]),                        # 27 buffers: two launches
+    (30, 60, 8, 8, True, "BF16", 30, None, 4, [2, 1, 9]),
+]
+
+
+@pytest.mark.parametrize("i", range(len(MIXED)))
+@pytest.mark.parametrize("padding", [0, 3])
+def test_prompts_and_single_tokens_in_one_write(ctx, i, padding):  # noqa: F811
+    base.test_new_tokens_are_turned_and_written(ctx, MIXED[i], padding)
