@@ -10,6 +10,7 @@ missing.
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -318,6 +319,7 @@ class StoreHandle:
         self.shape = shape
         self.name = name
         self.unique_id = B.load().mmr_store_id(handle)
+        ctx._handles.add(self)
 
     @property
     def devices(self) -> range:
@@ -328,20 +330,12 @@ class StoreHandle:
         return shard_bytes(self.shape)
 
 
-def _handle(a):
-    """The C handle of a store, plan or cache; None (which the C entry point refuses) if it was freed or destroyed, or went
-    with its context."""
-    return a._h if a._ctx._h is not None else None
-
-
-def _optional(a, what: str):
-    """The same for an argument that may be left out, where None would be taken for that."""
-    if a is None:
-        return None
-    h = _handle(a)
-    if h is None:
+def _given(a, what: str):
+    """The C handle of an argument that may be left out: one that was freed or destroyed has none, and None would be taken
+    for left out."""
+    if a._h is None:
         raise ValueError("%s was freed or destroyed" % what)
-    return h
+    return a._h
 
 
 _INT32_TYPES: dict = {}  # type objects of other packages -> whether they are int32 (their names are slow to make)
@@ -380,9 +374,10 @@ class RotaryPlan:
 
     def __init__(self, ctx: "ReshardContext", handle: C.c_void_p):
         self._ctx, self._h = ctx, handle
+        ctx._handles.add(self)
 
     def Destroy(self) -> None:
-        B.check(self._ctx._lib.mmr_rotary_destroy(_handle(self)))
+        B.check(self._ctx._lib.mmr_rotary_destroy(self._h))
         self._h = None
 
 
@@ -394,12 +389,13 @@ class PageCache:
 
     def __init__(self, ctx: "ReshardContext", handle: C.c_void_p):
         self._ctx, self._h, self._lib = ctx, handle, ctx._lib
+        ctx._handles.add(self)
 
     def _pairs(self, fn, a, b, what):
         (pa, na), (pb, nb) = _ids(self._ctx, a, what[0]), _ids(self._ctx, b, what[1])
         if na != nb:
             raise ValueError("%d %s, %d %s" % (na, what[0], nb, what[1]))
-        B.check(fn(_handle(self), pa, pb, na))
+        B.check(fn(self._h, pa, pb, na))
 
     def Extend(self, sequences, tokens) -> None:
         self._pairs(self._lib.mmr_pages_extend, sequences, tokens, ("sequences", "tokens"))
@@ -409,13 +405,13 @@ class PageCache:
 
     def Free(self, sequences) -> None:
         p, n = _ids(self._ctx, sequences, "sequences")
-        B.check(self._lib.mmr_pages_free(_handle(self), p, n))
+        B.check(self._lib.mmr_pages_free(self._h, p, n))
 
     def Copy(self, sources, destinations) -> None:
         self._pairs(self._lib.mmr_pages_copy, sources, destinations, ("sources", "destinations"))
 
     def Compact(self) -> None:
-        B.check(self._lib.mmr_pages_compact(_handle(self)))
+        B.check(self._lib.mmr_pages_compact(self._h))
 
     def Write(self, sequences, begins, k_pool: int, k: StoreHandle, v_pool: int = -1, v: Optional[StoreHandle] = None,
               rotary: Optional[RotaryPlan] = None, q: Optional[StoreHandle] = None, q_out: Optional[StoreHandle] = None) -> None:
@@ -423,18 +419,19 @@ class PageCache:
         (ps, n), (pb, nb) = _ids(self._ctx, sequences, "sequences"), _ids(self._ctx, begins, "begins")
         if nb != n + 1:
             raise ValueError("%d begins for %d sequences" % (nb, n))
-        B.check(self._lib.mmr_pages_write(_handle(self), ps, pb, n, k_pool, _handle(k), v_pool, _optional(v, "the v store"),
-                                          _optional(rotary, "the rotary plan"), _optional(q, "the q store"),
-                                          _optional(q_out, "the q_out store")))
+        B.check(self._lib.mmr_pages_write(self._h, ps, pb, n, k_pool, k._h, v_pool, None if v is None else _given(v, "the v store"),
+                                          None if rotary is None else _given(rotary, "the rotary plan"),
+                                          None if q is None else _given(q, "the q store"),
+                                          None if q_out is None else _given(q_out, "the q_out store")))
 
     def Status(self) -> Tuple[List[str], int]:
         """(reasons since the last Status, pages in use).  Blocks."""
         flags, used = C.c_uint32(), C.c_int64()
-        B.check(self._lib.mmr_pages_status(_handle(self), C.byref(flags), C.byref(used)))
+        B.check(self._lib.mmr_pages_status(self._h, C.byref(flags), C.byref(used)))
         return [name for name, bit in B.PAGES_FLAGS.items() if flags.value & bit], used.value
 
     def Destroy(self) -> None:
-        B.check(self._lib.mmr_pages_destroy(_handle(self)))
+        B.check(self._lib.mmr_pages_destroy(self._h))
         self._h = None
 
 
@@ -450,6 +447,7 @@ class ReshardContext:
     def __init__(self, hip_device: int = 0, hip_stream: Optional[int] = None):
         self._lib = B.load()
         self._h = C.c_void_p()
+        self._handles: weakref.WeakSet = weakref.WeakSet()  # stores, plans and caches, which end with the context
         self.hip_device = hip_device
         B.check(self._lib.mmr_context_create(hip_device, C.c_void_p(hip_stream) if hip_stream else None,
                                              C.byref(self._h)))
@@ -458,6 +456,8 @@ class ReshardContext:
         if self._h:
             self._lib.mmr_context_destroy(self._h)
             self._h = None
+            for handle in list(self._handles):
+                handle._h = None
 
     def __enter__(self):
         return self
@@ -617,9 +617,8 @@ class ReshardContext:
     def CreatePages(self, pools: Sequence[StoreHandle], table: StoreHandle, lengths: StoreHandle, refs: StoreHandle,
                     page_tokens: int) -> PageCache:
         h = C.c_void_p()
-        arr = (C.c_void_p * max(len(pools), 1))(*[_handle(p) for p in pools])
-        B.check(self._lib.mmr_pages_create(self._h, arr, len(pools), _handle(table), _handle(lengths), _handle(refs), page_tokens,
-                                           C.byref(h)))
+        arr = (C.c_void_p * max(len(pools), 1))(*[p._h for p in pools])
+        B.check(self._lib.mmr_pages_create(self._h, arr, len(pools), table._h, lengths._h, refs._h, page_tokens, C.byref(h)))
         return PageCache(self, h)
 
     def CreateRotary(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: Optional[str] = None,
@@ -639,8 +638,8 @@ class ReshardContext:
     def ApplyRotary(self, rotary: RotaryPlan, x: StoreHandle, out: Optional[StoreHandle] = None, seq_dim: int = 0,
                     positions: Optional[StoreHandle] = None, offset: int = 0, backward: bool = False) -> None:
         """Rows of x turned by their positions, into `out` (None: in place)."""
-        B.check(self._lib.mmr_rotary_apply(_handle(rotary), _handle(x), _handle(out if out is not None else x), seq_dim,
-                                           _optional(positions, "the positions store"), offset,
+        B.check(self._lib.mmr_rotary_apply(rotary._h, x._h, (out if out is not None else x)._h, seq_dim,
+                                           None if positions is None else _given(positions, "the positions store"), offset,
                                            B.MMR_ROTARY_BACKWARD if backward else 0))
 
     # -- measurement and inspection ----------------------------------------

@@ -1,6 +1,7 @@
 """Handles that are gone, in arguments that may be left out: refused, not taken for left out (no GPU: the C entry points are
 replaced by ones that note what they are given)."""
 import ctypes as C
+import weakref
 
 import pytest
 
@@ -25,18 +26,23 @@ def null(a):
     return a is None or (isinstance(a, C.c_void_p) and not a.value)
 
 
+def context(monkeypatch):
+    ctx = mm.ReshardContext.__new__(mm.ReshardContext)
+    ctx._lib, ctx._h, ctx._handles, ctx.hip_device = Noted(), C.c_void_p(8), weakref.WeakSet(), 0
+    monkeypatch.setattr(api.B, "load", lambda: ctx._lib)
+    return ctx
+
+
+def store(ctx, address):
+    return api.StoreHandle(ctx, C.c_void_p(address), None, "s")
+
+
 @pytest.fixture
 def world(monkeypatch):
-    ctx = mm.ReshardContext.__new__(mm.ReshardContext)
-    ctx._lib, ctx._h, ctx.hip_device = Noted(), C.c_void_p(8), 0
-
-    def store(address):
-        s = api.StoreHandle.__new__(api.StoreHandle)
-        s._ctx, s._h, s.name = ctx, C.c_void_p(address), "s"
-        return s
-
+    ctx = context(monkeypatch)
     w = dict(ctx=ctx, cache=api.PageCache(ctx, C.c_void_p(16)), plan=api.RotaryPlan(ctx, C.c_void_p(24)),
-             **{name: store(32 + 8 * i) for i, name in enumerate(("k", "v", "q", "q_out", "x", "out", "positions"))})
+             **{name: store(ctx, 32 + 8 * i) for i, name in enumerate(("k", "v", "q", "q_out", "x", "out", "positions"))})
+    ctx._lib.calls.clear()
     yield w
     ctx._h = None
 
@@ -69,38 +75,45 @@ def test_what_is_given_arrives(world):
                                        (write, ["k"]), (write, ["cache"]), (rotate, ["positions"]), (rotate, ["out"]), (rotate, ["x"]),
                                        (rotate, ["plan"])])
 @pytest.mark.parametrize("how", ["freed", "closed"])
-def test_what_is_gone_is_never_taken_for_left_out(world, call, gone, how):
-    """Freed or destroyed, or of a context that was closed: an error here, or null where the C entry point takes no null."""
-    ctx = world["ctx"]
-    if how == "freed":
+def test_what_is_gone_is_never_taken_for_left_out(world, monkeypatch, call, gone, how):
+    """Freed or destroyed, or of another context that was closed: an error here, or null where the C entry point takes no null."""
+    lib = world["ctx"]._lib
+    if how == "closed":
+        other = context(monkeypatch)
         for name in gone:
-            world[name]._h = None
-    else:
-        other = mm.ReshardContext.__new__(mm.ReshardContext)
-        other._h = None
-        for name in gone:
-            world[name]._ctx = other
+            world[name] = (api.RotaryPlan(other, C.c_void_p(80)) if name == "plan" else api.PageCache(other, C.c_void_p(80)) if name == "cache"
+                           else store(other, 80))
             if name == "cache":
-                world[name]._lib = ctx._lib
+                world[name]._lib = lib
+        other.close()
+    else:
+        for name in gone:
+            if name in ("plan", "cache"):
+                world[name].Destroy()
+            else:
+                world["ctx"].Free(world[name])
+    lib.calls.clear()
     needed = {write: {"cache": 0, "k": 5}, rotate: {"plan": 0, "x": 1, "out": 2}}[call]
     if set(gone) <= set(needed):
-        try:
-            call(world)
-        except ValueError:
-            return
-        (_, args), = ctx._lib.calls
+        call(world)
+        (_, args), = lib.calls
         assert all(null(args[needed[name]]) for name in gone)
     else:
         with pytest.raises(ValueError, match="freed|destroyed"):
             call(world)
-        assert not ctx._lib.calls
+        assert not lib.calls
 
 
 def test_calls_after_the_context_is_closed(world):
+    """Nothing that the context made reaches a C entry point."""
     ctx, cache, plan = world["ctx"], world["cache"], world["plan"]
-    ctx._h = None
     lib = ctx._lib
+    ctx.close()
+    ctx.close()
+    assert [name for name, _ in lib.calls] == ["mmr_context_destroy"]
+    lib.calls.clear()
     for call in (lambda: cache.Compact(), lambda: cache.Free((64, 1)), lambda: cache.Extend((64, 1), (72, 1)),
-                 lambda: cache.Status(), lambda: cache.Destroy(), lambda: plan.Destroy()):
+                 lambda: cache.Status(), lambda: cache.Destroy(), lambda: plan.Destroy(), lambda: ctx.Reshard(world["k"], world["v"])):
         call()
-    assert len(lib.calls) == 6 and all(null(args[0]) for _, args in lib.calls)
+    assert len(lib.calls) == 7 and all(null(args[0]) for _, args in lib.calls)
+    assert all(null(a) for a in lib.calls[-1][1])
