@@ -1289,7 +1289,6 @@ int context_check_store(mmr_context* ctx, const mmr_store* store, const char* wh
   return MMR_OK;
 }
 const Side& store_side(const mmr_store* store) { return store->side; }
-const mmr_sharded_shape& store_shape(const mmr_store* store) { return store->shape; }
 const std::string& store_key(const mmr_store* store) { return store->shape_key; }
 int64_t store_ordinal(const mmr_store* store) { return store->ordinal; }
 char* store_tile(const mmr_store* store, int64_t k) { return store->tile(k); }

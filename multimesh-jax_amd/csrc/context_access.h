@@ -50,7 +50,6 @@ mmr_store* context_find_store(mmr_context* ctx, int64_t id);  // null if it was 
 // The store is this context's and on the device.
 int context_check_store(mmr_context* ctx, const mmr_store* store, const char* what);
 const Side& store_side(const mmr_store* store);
-const mmr_sharded_shape& store_shape(const mmr_store* store);
 const std::string& store_key(const mmr_store* store);
 int64_t store_ordinal(const mmr_store* store);
 char* store_tile(const mmr_store* store, int64_t k);

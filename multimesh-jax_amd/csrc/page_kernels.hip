@@ -285,8 +285,9 @@ constexpr uint64_t kMaxMoveBlocks = 1u << 18;
 // bytes: 19.9 us, with a launch for the list 21.8; of 32,768: 30.1 and 23.7).
 constexpr int32_t kCompactWhole = 16384;
 // A copy of few pairs is one launch, whose workgroups (one a chunk) each check all pairs, up to so many workgroups times
-// pairs: 4 pairs of 1,024 chunks 4.6 us, in two launches 7.7; 16 of 1,024 5.5 and 7.5; 32 of 512 5.9 and 7.9; 32 of 2,048
-// 9.8 and 13.1; but 64 of 1,024 9.7 and 8.8, 32 of 8,192 32.5 and 29.2.
+// pairs: 4 pairs of 1,024 chunks 4.6 us, in two launches 7.7; 16 of 1,024 5.5 and 7.5; 32 of 512 5.9 and 7.9; but 64 of
+// 1,024 9.7 and 8.8, 32 of 8,192 32.5 and 29.2.  The product is a rough measure: 32 of 2,048, as many checks as 64 of 1,024,
+// would take 9.8 and go in two launches at 13.1.
 constexpr uint64_t kFewChecks = 48 * 1024;
 
 template <int KIND>
@@ -308,9 +309,9 @@ hipError_t launch_apply(const PageState& st, const PageWork& w, const PageMoveLa
 
 }  // namespace
 
-// Extend is one launch where no call of this size can give out more pages than its last workgroup writes in a few rounds;
-// else a second one follows, which does the writing if there is more (768 prompts of 128 pages each: 97 us by one
-// workgroup) and otherwise ends at once.
+// Extend is one launch (besides the scan's) where no call of this size can give out more pages than the plan's workgroup
+// writes in 16 rounds; else another one follows it, which does the writing if there is more than kExtendFew (768 prompts of
+// 128 pages each: 97 us by one workgroup) and otherwise ends at once.
 constexpr int64_t kExtendWhole = 16384;
 
 hipError_t launch_page_extend(const PageState& st, const PageWork& w, const int32_t* slots, const int32_t* counts, int32_t n,

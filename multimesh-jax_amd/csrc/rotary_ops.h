@@ -6,9 +6,10 @@
 // gradient of the input is the same with s of the other sign, as the matrix is m times a rotation.
 //
 // Angles.  f_i is held as a fraction of a turn in 64 bits of fixed point, so t modulo 1 is the low half of an integer
-// product and nothing is lost at far positions (2^-34 of a turn at position 2^31, where a 32-bit float product would be
-// off by many turns).  Its upper 32 bits are cut into a quarter turn and a rest within +-pi/4, and sine and cosine of
-// the rest are their Taylor sums to the 9th and 10th power: cut off under 2^-28, rounding 2^-24.
+// product, of which the upper 32 bits are used: low by under 2^-32 of a turn at any position, and up to 2^-34 off at position
+// 2^31 for the rounding of f_i, where a 32-bit float product would be off by many turns.  They are cut into a quarter turn
+// and a rest within +-pi/4, and sine and cosine of the rest are their Taylor sums to the 9th and 10th power: cut off under
+// 2^-28, rounding 2^-24.
 //
 // Bound: HBM; a row is read and written once.  The angles of a position are worked out once per lane and used for
 // several heads, so that their ~35 instructions a pair stay below the time of the memory traffic.
