@@ -535,8 +535,8 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  *
  * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
  * so on.  extend, fork and copy check all their entries first, fork the pages that are to be shared or copied too, and
- * change nothing at all if one is bad; the reason is
- * kept until mmr_pages_status reads it.  Pages are given out lowest free id first, in the order of the entries.
+ * change nothing at all if one is bad; the reason is kept until mmr_pages_status reads it.  free and compact leave what is
+ * out of step as it is, do the rest and tell.  Pages are given out lowest free id first, in the order of the entries.
  * MMR_PAGES_NONE in place of a sequence (fork: of the child; copy: of the destination) is no entry and is passed over, so
  * that a graph captured for the largest batch can be replayed for smaller ones.
  * ------------------------------------------------------------------------- */
@@ -604,9 +604,9 @@ int mmr_rotary_create(mmr_context* ctx, const mmr_rotary_options* options, mmr_r
 int mmr_rotary_destroy(mmr_rotary* rotary);
 
 /* out := x with its rows turned.  x and out: F32, BF16 or F16, rank 2 to 4, of one descriptor (out may be x itself, and
- * overlaps it in no other way; replicas of out may be adopted in one buffer, which is written once, and its tiles overlap in
- * no other way, which is refused); the last dim is the row, unsharded and minor-most, at least rotary_dim long, the rest of
- * it passes through.  Every other dim may be sharded, padded and laid out at will; padding is left alone.  The position
+ * overlaps it in no other way; replicas of out may be adopted in one buffer, which is written once, other tiles of out that
+ * overlap are refused); the last dim is the row, unsharded and minor-most, at least rotary_dim long, the rest of it passes
+ * through.  Every other dim may be sharded, padded and laid out at will; padding is left alone.  The position
  * of a row is offset + its index along seq_dim in the whole array, wherever its tile is, or what `positions` holds: an
  * S32 store [sequence], or [dim 0, sequence], whose tile on every device covers the sequence of x's tile there (sharded
  * alike, or replicated).  MMR_ROTARY_BACKWARD: out is the gradient of x where x holds the gradient of the result. */
@@ -620,9 +620,10 @@ int mmr_rotary_apply(mmr_rotary* rotary, mmr_store* x, mmr_store* out, int32_t s
  * are those of a sequence MMR_PAGES_NONE; the sequences are distinct (of two entries of one, either may be kept).  k
  * goes to pool k_pool, v (or NULL) to pool v_pool: stores [tokens, heads, dim], heads sharded as in the pool.  With a
  * rotary plan k is turned on its way, and q (any heads, [tokens, heads, dim], or NULL) is turned into q_out (or in
- * place; q_out and the pools overlap nothing else that the call reads or writes, so q_out is not k or v).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.  Tokens of an entry whose
- * sequence or page is not there, or that are more than the sequence holds, are left out (q_out too), the others are
- * written; the reason is kept for mmr_pages_status. */
+ * place; q_out and the pools overlap nothing else that the call reads or writes, so q_out is not k or v; replicas of
+ * q_out as in mmr_rotary_apply).  v, and k without a plan, move bit for bit, in any type.  All parts are of one type.
+ * Tokens of an entry whose sequence or page is not there, or that are more than the sequence holds, are left out (q_out
+ * too), the others are written; the reason is kept for mmr_pages_status. */
 int mmr_pages_write(mmr_pages* pages, const int32_t* sequences, const int32_t* begins, int32_t n, int32_t k_pool, mmr_store* k,
                     int32_t v_pool, mmr_store* v, mmr_rotary* rotary, mmr_store* q, mmr_store* q_out);
 
