@@ -535,8 +535,9 @@ int mmr_reshard_batch_plan_stats(mmr_context* ctx, mmr_store* const* srcs, mmr_s
  *
  * What the host cannot see is checked on the device: an entry that names no sequence or page, too few free pages, and
  * so on.  extend, fork and copy check all their entries first, fork the pages that are to be shared or copied too, and
- * change nothing at all if one is bad; the reason is kept until mmr_pages_status reads it.  free and compact leave what is
- * out of step as it is, do the rest and tell.  Pages are given out lowest free id first, in the order of the entries.
+ * change nothing at all if one is bad; the reason is kept until mmr_pages_status reads it.  free and compact leave
+ * pages that are out of step as they are, do the rest and tell.  Pages are given out lowest free id first, in the order
+ * of the entries.
  * MMR_PAGES_NONE in place of a sequence (fork: of the child; copy: of the destination) is no entry and is passed over, so
  * that a graph captured for the largest batch can be replayed for smaller ones.
  * ------------------------------------------------------------------------- */

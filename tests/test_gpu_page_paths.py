@@ -1,5 +1,7 @@
 """Page operators on the GPU where a call takes another form than small ones do (more launches, more segments of pages, more
 chunks), on both sides of each limit, and on tables that are out of step with themselves."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -387,3 +389,53 @@ MIXED = [
 @pytest.mark.parametrize("padding", [0, 3])
 def test_prompts_and_single_tokens_in_one_write(ctx, i, padding):  # noqa: F811
     base.test_new_tokens_are_turned_and_written(ctx, MIXED[i], padding)
+
+
+@pytest.mark.parametrize("form", ["a launch checks", "a launch checks and scans"])
+def test_the_longer_forms_replay_from_a_hip_graph(form):
+    """fork with its check in a launch of its own, a planned copy and a compact, captured once: replays that are carried out
+    and one whose fork is refused for a bad row, with eager calls in between."""
+    hip = base.hip_graph_functions()
+    with mm.ReshardContext(0) as c:
+        size = dict(FORKS[form])
+        size["P"] = max(size["P"], 400)
+        p = Pair(c, S=24, T=4, shape=(4, 2, 8), type="BF16", seed=9, **size)
+        m, rng = p.model, np.random.Generator(np.random.PCG64(9))
+        p.op("extend", np.arange(6), [14, 9, 20, 1, 16, 7])
+        arrays = {k: p.ids(np.zeros(n)) for k, n in dict(parents=3, children=3, src=70, dst=70).items()}
+        c.Sync()
+        graph, exe = C.c_void_p(), C.c_void_p()
+        assert hip.hipStreamBeginCapture(c.stream, 0) == 0
+        p.cache.Fork(arrays["parents"], arrays["children"])
+        p.cache.Copy(arrays["src"], arrays["dst"])
+        p.cache.Compact()
+        assert hip.hipStreamEndCapture(c.stream, C.byref(graph)) == 0 and graph.value
+        assert hip.hipGraphInstantiate(C.byref(exe), graph, None, None, 0) == 0
+        for replay in range(4):
+            parents, children = rng.choice(np.flatnonzero(m.lengths > 0), 3), np.flatnonzero(m.lengths == 0)[:3]
+            if replay == 2:
+                parents[1] = 0
+            ids = rng.permutation(np.arange(100, 400))
+            for name, v in (("parents", parents), ("children", children), ("src", ids[70:140]), ("dst", ids[:70])):
+                c.AssembleShards(arrays[name].shape, 0, np.asarray(v, np.int32).view(np.uint8), existing_store=arrays[name])
+            say("graph of the longer forms, %s, replay %d" % (form, replay))
+            if replay == 2:  # the first, full page of one parent is not there
+                held = m.table[0, 0]
+                m.table[0, 0] = m.P
+                put(p, "table")
+            assert hip.hipGraphLaunch(exe, c.stream) == 0
+            if replay == 2:
+                m.table[0, 0] = held
+                m.copy(ids[70:140], ids[:70])
+                m.compact()
+                assert p.cache.Status()[0] == ["BAD_PAGE"]
+                assert p.tables()[0][0, 0] == m.P  # compact leaves it too; the page itself is where the model has it
+                put(p, "table")
+            else:
+                m.fork(parents, children)
+                m.copy(ids[70:140], ids[:70])
+                m.compact()
+            p.check()
+            p.op("free", [int(np.flatnonzero(m.lengths > 0)[-1])])  # eager, between the replays
+            p.check()
+        assert hip.hipGraphExecDestroy(exe) == 0 and hip.hipGraphDestroy(graph) == 0
